@@ -39,7 +39,9 @@ typedef void* mgpu_stream_t;
 /* Value types (operators.hxx:91-124 are templates over the value type). */
 enum {
   MGPU_I32 = 0, MGPU_U32 = 1, MGPU_I64 = 2, MGPU_U64 = 3,
-  MGPU_F32 = 4, MGPU_F64 = 5
+  MGPU_F32 = 4, MGPU_F64 = 5,
+  /* rows only (embedding, distillation, sampling): IEEE half and bfloat16 */
+  MGPU_F16 = 6, MGPU_BF16 = 7
 };
 /* mgpu::plus_t, mgpu::maximum_t, mgpu::minimum_t (operators.hxx:91-124). */
 enum { MGPU_PLUS = 0, MGPU_MAXIMUM = 1, MGPU_MINIMUM = 2 };
@@ -336,6 +338,99 @@ MGPU_HIP_API size_t mgpu_hip_inner_join_pairs_workspace_bytes(int a_count,
   int64_t join_count);
 MGPU_HIP_API int mgpu_hip_inner_join_pairs(int a_count, int b_count,
   int join_count, const void* count_workspace, int* pairs, void* workspace,
+  size_t workspace_bytes, mgpu_stream_t stream);
+
+/* ---- between tokens and rows -------------------------------------------- */
+
+/* The functions below have no counterpart in moderngpu, whose values are
+ * scalars: they are its gathers, segmented sums, reductions and searches with
+ * rows of values, as language models use them at both ends of a vocabulary.
+ *  - dtype is MGPU_F32, MGPU_F16 or MGPU_BF16.  Sums are held in 32 bits
+ *    (64 where it says so); a result is rounded to its type once.
+ *  - A matrix is a pointer to its first value and a stride in values from one
+ *    row to the next.  Inputs take any stride >= 0 (0: the same row again);
+ *    an output's is at least its row length.  Pointers are aligned to one
+ *    value, nothing more.
+ *  - An output may not overlap an input, except where it says so. */
+
+/* output[t] = scale * table[ids[t]] for t in [0, count): rows of dim values.
+ * An id outside [0, num_rows) is padding and gives zeros. */
+MGPU_HIP_API int mgpu_hip_embedding_lookup(const void* table, int num_rows,
+  int dim, int64_t table_stride, const int* ids, int count, float scale,
+  void* output, int64_t output_stride, int dtype, mgpu_stream_t stream);
+
+/* The lookup's gradient.  accumulate == 0: output[v] = scale * sum of grad[t]
+ * over the t with ids[t] == v, for every row v in [0, num_rows).  Otherwise
+ * that is added to output[v] for the rows that occur, and the others are
+ * neither read nor written.  ids outside [0, num_rows) add to nothing.  The
+ * order of the additions depends on the sizes and the ids alone.
+ * output_dtype is grad_dtype or MGPU_F32.  Workspace:
+ * mgpu_hip_embedding_grad_workspace_bytes (0 for sizes that are refused). */
+MGPU_HIP_API size_t mgpu_hip_embedding_grad_workspace_bytes(int count,
+  int num_rows, int dim);
+MGPU_HIP_API int mgpu_hip_embedding_grad(const void* grad,
+  int64_t grad_stride, const int* ids, int count, int num_rows, int dim,
+  float scale, int accumulate, void* output, int64_t output_stride,
+  int grad_dtype, int output_dtype, void* workspace, size_t workspace_bytes,
+  mgpu_stream_t stream);
+
+/* Distillation from a teacher's top logits, one loss a row.  Row r has
+ * logits z[0 .. vocab), `top` teacher entries (teacher_ids[r * top + k],
+ * teacher_logits[r * top + k]; 0 <= top <= MGPU_HIP_DISTILL_MAX_TOP) and
+ * weight w = weights[r] (weights == NULL: 1).  With
+ * p = softmax(a / temperature) over the entries whose id lies in [0, vocab)
+ * (the others are padding) and q = softmax(z / temperature):
+ *   loss[r] = w * temperature^2 * sum_k p_k (log p_k - log q[id_k])
+ *   dz[v]   = w * temperature * (q[v] - sum of p_k over id_k == v)
+ * Several entries may name one id.  A row of weight 0, or without a usable
+ * entry, is not read: loss 0, gradient 0, norms 0.  A row of -inf only has
+ * q = 0; NaN or +inf in a row make its loss and gradient NaN.
+ * teacher_dtype: MGPU_F32, MGPU_F16 or MGPU_BF16.  temperature > 0, finite.
+ *
+ * norms (2 floats a row: the largest logit, and log sum exp((z - largest) /
+ * temperature)) is what distill_grad takes; it may be NULL in distill_loss.
+ * distill_grad's weights are the loss's times the gradient that arrives at
+ * each row's loss.  grad may be the logits themselves (same pointer and
+ * stride). */
+#define MGPU_HIP_DISTILL_MAX_TOP 1024
+MGPU_HIP_API int mgpu_hip_distill_loss(const void* logits,
+  int64_t logits_stride, int rows, int vocab, const int* teacher_ids,
+  const void* teacher_logits, int top, float temperature,
+  const float* weights, float* loss, float* norms, int dtype,
+  int teacher_dtype, mgpu_stream_t stream);
+MGPU_HIP_API int mgpu_hip_distill_grad(const void* logits,
+  int64_t logits_stride, int rows, int vocab, const float* norms,
+  const int* teacher_ids, const void* teacher_logits, int top,
+  float temperature, const float* weights, void* grad, int64_t grad_stride,
+  int dtype, int teacher_dtype, mgpu_stream_t stream);
+MGPU_HIP_API int mgpu_hip_distill_loss_and_grad(const void* logits,
+  int64_t logits_stride, int rows, int vocab, const int* teacher_ids,
+  const void* teacher_logits, int top, float temperature,
+  const float* weights, float* loss, void* grad, int64_t grad_stride,
+  int dtype, int teacher_dtype, mgpu_stream_t stream);
+
+/* One token a row from its logits and uniform[row] in [0, 1).  With a row's
+ * logits ordered by value, largest first, equal ones by index: top-k keeps
+ * the first top_k (<= 0: all); top-p keeps, with p = softmax(z / temperature)
+ * over those, every one whose predecessors' p sum up to less than top_p, and
+ * always the first (>= 1: all); min-p keeps every p of at least min_p times
+ * the largest.  token[row] is the first index, in order of index, at which
+ * the running sum of the kept p exceeds uniform[row] times their total;
+ * logprob[row] is the logarithm of its share of that total.  temperature
+ * <= 0 keeps the first alone.  -inf and NaN are never drawn, +inf counts as
+ * the largest finite float; a row with nothing else gives token -1 and
+ * logprob -inf.  Probabilities are summed as 64-bit whole numbers: the token
+ * does not depend on the order of the sums.
+ * Each setting is an array with a value a row or, where that is NULL, the
+ * one value for all rows.  vocab in [1, MGPU_HIP_SAMPLE_MAX_VOCAB].
+ * Workspace: mgpu_hip_sample_workspace_bytes. */
+#define MGPU_HIP_SAMPLE_MAX_VOCAB (1 << 24)
+MGPU_HIP_API size_t mgpu_hip_sample_workspace_bytes(int rows, int vocab);
+MGPU_HIP_API int mgpu_hip_sample(const void* logits, int64_t logits_stride,
+  int rows, int vocab, const float* uniform, const float* temperature,
+  const int* top_k, const float* top_p, const float* min_p,
+  float temperature_all, int top_k_all, float top_p_all, float min_p_all,
+  int* token, float* logprob, int dtype, void* workspace,
   size_t workspace_bytes, mgpu_stream_t stream);
 
 #ifdef __cplusplus

@@ -1,0 +1,85 @@
+// mgpu for AMD CDNA4: access to rows of 32- and 16-bit floating-point values,
+// shared by the operators between tokens and rows (kernel_embedding.hxx,
+// kernel_distill.hxx, kernel_sample.hxx).  No counterpart in moderngpu, whose
+// values are scalars.
+//
+// A row is `dim` consecutive values that start at any multiple of the value's
+// own size: rows of odd length put most starts off every vector boundary.
+// gfx950 moves 16 bytes from or to any address in one instruction, so every
+// row is walked in 16-byte chunks counted from its own start, and only the
+// chunk that would cross the row's end goes value by value.
+#pragma once
+#include <type_traits>
+#include "intrinsics.hxx"
+#include "transform.hxx"
+
+BEGIN_MGPU_NAMESPACE
+
+typedef _Float16 f16_t;
+typedef __bf16 bf16_t;
+
+namespace detail {
+
+typedef unsigned row_words_t __attribute__((ext_vector_type(4)));
+// The same 16 bytes at an address that is aligned to 2 or 4 of them only.
+typedef row_words_t row_words_any2_t __attribute__((aligned(2)));
+typedef row_words_t row_words_any4_t __attribute__((aligned(4)));
+
+template<typename type_t>
+struct row_chunk_t {
+  enum { width = 16 / sizeof(type_t) };
+  typedef typename std::conditional<2 == sizeof(type_t), row_words_any2_t,
+    row_words_any4_t>::type any_words_t;
+
+  type_t x[width];
+
+  MGPU_DEVICE void load_all(const type_t* p) {
+    row_words_t w = *(const any_words_t*)p;
+    __builtin_memcpy(x, &w, 16);
+  }
+  // The first n values; `rest` in the others.
+  MGPU_DEVICE void load(const type_t* p, int n, type_t rest) {
+    if(n >= width) load_all(p);
+    else {
+      PRAGMA_UNROLL
+      for(int i = 0; i < width; ++i) x[i] = i < n ? p[i] : rest;
+    }
+  }
+  MGPU_DEVICE void store_all(type_t* p) const {
+    row_words_t w;
+    __builtin_memcpy(&w, x, 16);
+    *(any_words_t*)p = w;
+  }
+  MGPU_DEVICE void store(type_t* p, int n) const {
+    if(n >= width) store_all(p);
+    else {
+      PRAGMA_UNROLL
+      for(int i = 0; i < width; ++i) if(i < n) p[i] = x[i];
+    }
+  }
+};
+
+struct float_max_t {
+  MGPU_HOST_DEVICE float operator()(float a, float b) const {
+    return __builtin_fmaxf(a, b);
+  }
+};
+
+// Fold of x over the CTA's nt threads, returned to all of them; the same for
+// every call with the same values, in whatever order the waves arrive.
+// `shared` may be used again behind the next barrier.
+template<int nt, typename type_t, typename op_t>
+MGPU_DEVICE type_t cta_allreduce(type_t x, op_t op, int tid,
+  type_t (&shared)[nt / 64]) {
+  x = wave_allreduce(x, op, tid & 63);
+  if(!(tid & 63)) shared[tid / 64] = x;
+  __syncthreads();
+  type_t y = shared[0];
+  PRAGMA_UNROLL
+  for(int i = 1; i < nt / 64; ++i) y = op(y, shared[i]);
+  return y;
+}
+
+} // namespace detail
+
+END_MGPU_NAMESPACE

@@ -15,4 +15,7 @@ from .ops import (  # noqa: F401
     sorted_search, inner_join, prepare_segreduce, prepare_load_balance_search,
     segreduce_static,
 )
+from .rows import (  # noqa: F401
+    embedding_lookup, embedding_grad, distill_loss, distill_grad, distill_loss_and_grad, sample,
+)
 from ._native import lib, library_path  # noqa: F401

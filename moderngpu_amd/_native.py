@@ -7,6 +7,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _SO = os.path.join(_HERE, "libmgpu_hip.so")
 
 c_int, c_i64, c_size, c_vp = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
+c_f32 = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/mgpu_hip.h.
 SIGNATURES = {
@@ -47,6 +48,14 @@ SIGNATURES = {
     "mgpu_hip_inner_join_count": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_vp, c_size, c_vp]),
     "mgpu_hip_inner_join_pairs_workspace_bytes": (c_size, [c_int, c_i64]),
     "mgpu_hip_inner_join_pairs": (c_int, [c_int, c_int, c_int, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "mgpu_hip_embedding_lookup": (c_int, [c_vp, c_int, c_int, c_i64, c_vp, c_int, c_f32, c_vp, c_i64, c_int, c_vp]),
+    "mgpu_hip_embedding_grad_workspace_bytes": (c_size, [c_int, c_int, c_int]),
+    "mgpu_hip_embedding_grad": (c_int, [c_vp, c_i64, c_vp, c_int, c_int, c_int, c_f32, c_int, c_vp, c_i64, c_int, c_int, c_vp, c_size, c_vp]),
+    "mgpu_hip_distill_loss": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_vp, c_int, c_f32, c_vp, c_vp, c_vp, c_int, c_int, c_vp]),
+    "mgpu_hip_distill_grad": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_f32, c_vp, c_vp, c_i64, c_int, c_int, c_vp]),
+    "mgpu_hip_distill_loss_and_grad": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_vp, c_int, c_f32, c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_vp]),
+    "mgpu_hip_sample_workspace_bytes": (c_size, [c_int, c_int]),
+    "mgpu_hip_sample": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_f32, c_int, c_f32, c_f32, c_vp, c_vp, c_int, c_vp, c_size, c_vp]),
     "mgpu_hip_workcreate_workspace_bytes": (c_size, [c_int, c_int]),
     "mgpu_hip_workcreate_upsweep": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_vp, c_size, c_vp]),
     "mgpu_hip_workcreate_downsweep": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
