@@ -65,28 +65,40 @@ def test_distill_refuses(mem):
     good = dict(z=p[0], zs=16, rows=3, vocab=16, ids=p[1], a=p[2], top=4, tau=1.0, w=p[3], loss=p[4], norms=p[5],
                 grad=p[6], gs=16, dt=F16, tt=F32)
 
-    def calls(**kw):
+    # Each entry point by itself: a call that is not refused would launch a
+    # kernel on these addresses where there is a GPU.
+    def args(kw):
         a = dict(good, **kw)
-        front = (a["z"], a["zs"], a["rows"], a["vocab"])
-        teacher = (a["ids"], a["a"], a["top"], a["tau"], a["w"])
-        back = (a["dt"], a["tt"], None)
-        return (L.mgpu_hip_distill_loss(*front, *teacher, a["loss"], a["norms"], *back),
-                L.mgpu_hip_distill_grad(*front, a["norms"], *teacher, a["grad"], a["gs"], *back),
-                L.mgpu_hip_distill_loss_and_grad(*front, *teacher, a["loss"], a["grad"], a["gs"], *back))
+        return (a, (a["z"], a["zs"], a["rows"], a["vocab"]), (a["ids"], a["a"], a["top"], a["tau"], a["w"]),
+                (a["dt"], a["tt"], None))
+
+    def loss(**kw):
+        a, front, teacher, back = args(kw)
+        return L.mgpu_hip_distill_loss(*front, *teacher, a["loss"], a["norms"], *back)
+
+    def grad(**kw):
+        a, front, teacher, back = args(kw)
+        return L.mgpu_hip_distill_grad(*front, a["norms"], *teacher, a["grad"], a["gs"], *back)
+
+    def both(**kw):
+        a, front, teacher, back = args(kw)
+        return L.mgpu_hip_distill_loss_and_grad(*front, *teacher, a["loss"], a["grad"], a["gs"], *back)
+
     for bad in (dict(rows=-1), dict(vocab=-1), dict(top=-1), dict(top=1025), dict(tau=0.0), dict(tau=-1.0),
                 dict(tau=float("nan")), dict(tau=float("inf")), dict(tau=1e-39), dict(tau=1e30), dict(zs=-1), dict(dt=F64), dict(tt=F64),
                 dict(z=None), dict(ids=None), dict(a=None), dict(z=p[0] + 1), dict(w=p[3] + 2)):
-        assert calls(**bad) == (INVALID,) * 3, bad
-    loss, grad, both = calls(loss=None, grad=None)
-    assert loss == grad == both == INVALID
-    assert calls(gs=15)[1:] == (INVALID,) * 2                     # rows that overlap
-    assert calls(grad=p[0] + 2)[1:] == (INVALID,) * 2             # neither apart from the logits nor the same
-    assert calls(grad=p[0], gs=17)[1:] == (INVALID,) * 2
-    assert calls(grad=p[1])[1:] == (INVALID,) * 2
-    assert calls(loss=p[0])[0] == calls(loss=p[0])[2] == INVALID
-    assert calls(loss=p[5])[0] == INVALID                         # loss and norms
-    assert calls(norms=None)[1] == INVALID
-    assert calls(rows=0) == (0, 0, 0)
+        for call in (loss, grad, both):
+            assert call(**bad) == INVALID, bad
+    for bad in (dict(gs=15), dict(grad=None), dict(grad=p[0] + 2),      # rows that overlap; neither apart from the logits nor the same
+                dict(grad=p[0], gs=17), dict(grad=p[1])):
+        for call in (grad, both):
+            assert call(**bad) == INVALID, bad
+    for bad in (dict(loss=None), dict(loss=p[0])):
+        for call in (loss, both):
+            assert call(**bad) == INVALID, bad
+    assert loss(loss=p[5]) == INVALID                             # loss and norms
+    assert grad(norms=None) == INVALID
+    assert loss(rows=0) == grad(rows=0) == both(rows=0) == 0
 
 
 def test_sample_refuses(mem):
