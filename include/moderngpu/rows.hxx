@@ -9,7 +9,6 @@
 // row is walked in 16-byte chunks counted from its own start, and only the
 // chunk that would cross the row's end goes value by value.
 #pragma once
-#include <type_traits>
 #include "intrinsics.hxx"
 #include "transform.hxx"
 
@@ -21,20 +20,25 @@ typedef __bf16 bf16_t;
 namespace detail {
 
 typedef unsigned row_words_t __attribute__((ext_vector_type(4)));
-// The same 16 bytes at an address that is aligned to 2 or 4 of them only.
-typedef row_words_t row_words_any2_t __attribute__((aligned(2)));
-typedef row_words_t row_words_any4_t __attribute__((aligned(4)));
+// The same 16 bytes at an address that is aligned to 2 or 4 of them only (an
+// alignment on a typedef would be dropped where it goes through a template).
+template<int alignment> struct row_words_at_t;
+template<> struct __attribute__((packed, aligned(2))) row_words_at_t<2> {
+  row_words_t w;
+};
+template<> struct __attribute__((packed, aligned(4))) row_words_at_t<4> {
+  row_words_t w;
+};
 
 template<typename type_t>
 struct row_chunk_t {
   enum { width = 16 / sizeof(type_t) };
-  typedef typename std::conditional<2 == sizeof(type_t), row_words_any2_t,
-    row_words_any4_t>::type any_words_t;
+  typedef row_words_at_t<sizeof(type_t)> any_words_t;
 
   type_t x[width];
 
   MGPU_DEVICE void load_all(const type_t* p) {
-    row_words_t w = *(const any_words_t*)p;
+    row_words_t w = ((const any_words_t*)p)->w;
     __builtin_memcpy(x, &w, 16);
   }
   // The first n values; `rest` in the others.
@@ -48,7 +52,7 @@ struct row_chunk_t {
   MGPU_DEVICE void store_all(type_t* p) const {
     row_words_t w;
     __builtin_memcpy(&w, x, 16);
-    *(any_words_t*)p = w;
+    ((any_words_t*)p)->w = w;
   }
   MGPU_DEVICE void store(type_t* p, int n) const {
     if(n >= width) store_all(p);

@@ -38,13 +38,15 @@ int mgpu_hip_sample(const void* logits, int64_t logits_stride, int rows,
   }
   if(out[0].overlaps(out[1])) return (int)hipErrorInvalidValue;
   size_t need = mgpu_hip_sample_workspace_bytes(rows, vocab);
-  if(need && (!workspace || workspace_bytes < need))
+  if(need && (!workspace || workspace_bytes < need ||
+    (uintptr_t)workspace % 8 || !detail::sample_grid_ok(rows, vocab)))
     return (int)hipErrorInvalidValue;
   return with_row_type(dtype, [&](auto* p) {
     return guarded(stream, [&](context_t& context) {
       detail::sample_launch((decltype(p))logits, logits_stride, rows, vocab,
-        uniform, temperature, top_k, top_p, min_p, temperature_all, top_k_all,
-        top_p_all, min_p_all, token, logprob, workspace, context);
+        uniform, detail::sample_settings_t { temperature, top_k, top_p, min_p,
+          temperature_all, top_k_all, top_p_all, min_p_all }, token, logprob,
+        workspace, context);
     });
   });
 }
