@@ -172,6 +172,13 @@ MGPU_DEVICE inline void needed_here(const type_t& x) {
   asm volatile("" :: "v"(s.w[0]));
 }
 
+// Makes a constant a value in a vector register: what is added to a product
+// of 64-bit floats is otherwise moved there word by word before each use.
+MGPU_DEVICE inline double held_in_register(double x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 template<typename type_t>
 MGPU_DEVICE inline type_t bpermute(type_t x, int src_lane) {
   lane_words_t<type_t> s(x);

@@ -51,26 +51,32 @@ MGPU_HOST_DEVICE float sample_value(unsigned key) {
 }
 
 // 2^y for y <= 0 to 4e-14, relative: y = n + f with |f| <= 1/2, and 2^f by
-// the polynomial that interpolates (2^f - 1) / f at 9 Chebyshev nodes.
-MGPU_DEVICE inline double sample_exp2(double y) {
-  const double magic = 6755399441055744.;             // 1.5 * 2^52
-  y = __builtin_fmax(y, -1100.);
-  double t = y + magic;
-  double f = y - (t - magic);
-  double x = 1.0203121063391729e-07;
-  x = __builtin_fma(x, f, 1.3255224878668817e-06);
-  x = __builtin_fma(x, f, 1.525268684626772e-05);
-  x = __builtin_fma(x, f, 0.00015403455852453838);
-  x = __builtin_fma(x, f, 0.0013333558179043112);
-  x = __builtin_fma(x, f, 0.0096181291594025584);
-  x = __builtin_fma(x, f, 0.055504108664760424);
-  x = __builtin_fma(x, f, 0.24022650695812989);
-  x = __builtin_fma(x, f, 0.69314718055994529);
-  x = __builtin_fma(x, f, 1.);
-  long long bits;
-  __builtin_memcpy(&bits, &t, 8);
-  return __builtin_amdgcn_ldexp(x, (int)bits);
-}
+// the polynomial that interpolates (2^f - 1) / f at 9 Chebyshev nodes.  NaN
+// (0 times infinity) gives 0.
+struct sample_exp2_t {
+  double a[8];
+
+  __forceinline__ MGPU_DEVICE sample_exp2_t() {
+    const double c[8] = { 1.3255224878668817e-06, 1.525268684626772e-05,
+      0.00015403455852453838, 0.0013333558179043112, 0.0096181291594025584,
+      0.055504108664760424, 0.24022650695812989, 0.69314718055994529 };
+    PRAGMA_UNROLL
+    for(int i = 0; i < 8; ++i) a[i] = held_in_register(c[i]);
+  }
+  __forceinline__ MGPU_DEVICE double operator()(double y) const {
+    const double magic = 6755399441055744.;           // 1.5 * 2^52
+    y = __builtin_fmax(y, -1100.);
+    double t = y + magic;
+    double f = y - (t - magic);
+    double x = 1.0203121063391729e-07;
+    PRAGMA_UNROLL
+    for(int i = 0; i < 8; ++i) x = __builtin_fma(x, f, a[i]);
+    x = __builtin_fma(x, f, 1.);
+    long long bits;
+    __builtin_memcpy(&bits, &t, 8);
+    return __builtin_amdgcn_ldexp(x, (int)bits);
+  }
+};
 
 // One row's settings.
 struct sample_row_t {
@@ -79,7 +85,7 @@ struct sample_row_t {
   int k;
   double p, least;
   bool by_count, by_mass;
-  MGPU_DEVICE bool all() const { return !by_count && !by_mass && !(least > 0); }
+  __forceinline__ MGPU_DEVICE bool all() const { return !by_count && !by_mass && !(least > 0); }
 };
 struct sample_settings_t {
   const float* temperature;
@@ -90,7 +96,7 @@ struct sample_settings_t {
   int top_k_all;
   float top_p_all, min_p_all;
 
-  MGPU_DEVICE sample_row_t row(int r, int vocab) const {
+  __forceinline__ MGPU_DEVICE sample_row_t row(int r, int vocab) const {
     sample_row_t s;
     float t = temperature ? temperature[r] : temperature_all;
     s.k = top_k ? top_k[r] : top_k_all;
@@ -121,7 +127,7 @@ enum { sample_piece_nt = 256, sample_piece = 8192, sample_bins = 64,
 struct sample_piece_t {
   double sum;                   // of 2^((z - max) c)
   double segments[sample_segments];   // the same by 64 chunks of tokens
-  float table[sample_bins];     // the same by half octaves below max
+  int table[sample_bins];       // tokens by half octaves of it below max
   float max;
   int listed;                   // candidates; more than sample_list: too many
   unsigned short list[sample_list];   // where they are in the piece
@@ -133,11 +139,13 @@ struct sample_piece_t {
 //              1024 groups of 8 tokens are counted in 64 bins between the
 //              largest and the smallest of them; the first bins that hold k
 //              maxima hold the piece's k largest tokens, and little else.
-//   top-p      the sum of its probabilities and their sums by half octaves,
-//              from which the row learns how far down the kept ones reach
+//   top-p      the sum of its probabilities, and how many tokens there are in
+//              each half octave, which brackets how far down the kept ones
+//              reach.  (Sums by half octave would bracket it closer, but an
+//              LDS addition of floats takes 200 cycles a wave, a count 4.)
 //   neither    the sum, and the sums of short runs of tokens.
-// A 64-bit exponential is 17 instructions a token and what bounds the last
-// two: 131072 x 256 tokens take 15 us of every SIMD's time.
+// The last two are bound by the 64-bit exponential, some 25 instructions a
+// token.
 template<typename type_t>
 struct sample_piece_f {
   const type_t* logits;
@@ -157,7 +165,7 @@ struct sample_piece_f {
       groups = items / 8 };
     typedef row_chunk_t<type_t> chunk_t;
     const float inf = __builtin_inff();
-    __shared__ float shared_table[sample_bins][64];
+    __shared__ int shared_table[sample_bins][64];
     __shared__ int shared_hist[sample_bins];
     __shared__ float shared_max[waves], shared_min[waves];
     __shared__ double shared_sum[waves];
@@ -199,8 +207,7 @@ struct sample_piece_f {
       return;
     }
 
-    if(s.by_count) {
-      if(s.k > sample_max_k) return;
+    if(s.by_count && s.k <= sample_max_k) {
       // Nothing further below than this has a probability left: 52 octaves.
       float low = m - 104.f / s.c2;
       float least = m;
@@ -245,26 +252,35 @@ struct sample_piece_f {
       return;
     }
 
-    bool all = s.all();
-    if(!s.by_mass && !all) return;
-    if(s.by_mass) {
+    bool all = s.all(), count = s.by_count || s.by_mass;
+    if(!all && !count) return;
+    if(count) {
       for(int i = tid; i < sample_bins * 64; i += nt)
         (&shared_table[0][0])[i] = 0;
       __syncthreads();
+      // Every lane has a column of the table: no two add at one address.
+      PRAGMA_UNROLL
+      for(int i = 0; i < items; ++i)
+        if(z[i] > -inf)
+          atomicAdd(&shared_table[bin_of((m - z[i]) * s.c2)][lane], 1);
+      __syncthreads();
+      // Four threads a bin.
+      int bin = tid / 4, n = 0;
+      for(int i = 0; i < 16; ++i)
+        n += shared_table[bin][(tid & 3) * 16 + ((i + bin) & 15)];
+      n += dpp_move<dpp_quad_xor1>(n, n);
+      n += dpp_move<dpp_quad_xor2>(n, n);
+      if(!(tid & 3)) mine.table[bin] = n;
+      if(s.by_count) return;
     }
+    sample_exp2_t exp2;
     double sum = 0;
     PRAGMA_UNROLL
     for(int c = 0; c < chunks; ++c) {
       double part = 0;
       PRAGMA_UNROLL
-      for(int i = c * W; i < c * W + W; ++i) {
-        double e = sample_exp2(((double)z[i] - (double)m) * s.c);
-        if(!(z[i] > -inf)) e = 0;
-        part += e;
-        // Every lane has a column of the table: no two add at one address.
-        if(s.by_mass)
-          atomicAdd(&shared_table[bin_of((m - z[i]) * s.c2)][lane], (float)e);
-      }
+      for(int i = c * W; i < c * W + W; ++i)
+        part += exp2(((double)z[i] - (double)m) * s.c);
       if(all) {
         part = wave_allreduce(part, plus_t<double>(), lane);
         if(!lane) mine.segments[c * waves + tid / 64] = part;
@@ -279,27 +295,30 @@ struct sample_piece_f {
       for(int w = 1; w < waves; ++w) sum += shared_sum[w];
       mine.sum = sum;
     }
-    if(s.by_mass) {
-      // Four threads a bin.
-      int bin = tid / 4;
-      float x = 0;
-      for(int i = 0; i < 16; ++i)
-        x += shared_table[bin][(tid & 3) * 16 + ((i + bin) & 15)];
-      x += dpp_move<dpp_quad_xor1>(x, x);
-      x += dpp_move<dpp_quad_xor2>(x, x);
-      if(!(tid & 3)) mine.table[bin] = x;
-    }
   }
 };
 
-// One CTA per row finishes it, on a list of candidates in LDS where the kept
-// tokens are few, and otherwise on the row itself.
-enum { sample_nt = 1024, sample_candidates = 16384 };
+// One CTA per row finishes it.  Where the tokens that may be kept are few, they
+// are listed in LDS and everything happens on the list.  Otherwise the row is
+// read again: a border found by top-k or top-p is first bracketed by the counts
+// per half octave, the tokens above the bracket are added up, those inside are
+// listed, and the border is found among them.
+enum { sample_nt = 1024, sample_candidates = 16384, sample_row_bins = 128 };
+
+// Which tokens are kept: those with a larger key, and of those with this one
+// the ones up to `last`.
+struct sample_cut_t {
+  unsigned key;
+  int last;
+  __forceinline__ MGPU_DEVICE bool keeps(unsigned k, int v) const {
+    return k > key || (k == key && v <= last);
+  }
+};
 
 template<typename type_t>
 struct sample_row_f {
   enum { nt = sample_nt, num_waves = nt / 64,
-    W = row_chunk_t<type_t>::width,
+    W = row_chunk_t<type_t>::width, per_thread = 16, unroll = per_thread / W,
     // Bits that a key has below those of the logits' type.
     key_shift = sizeof(type_t) == 4 ? 0 :
       std::is_same<type_t, f16_t>::value ? 13 : 16 };
@@ -315,17 +334,15 @@ struct sample_row_f {
   float* logprob;
 
   struct shared_t {
-    union {
-      struct {
-        unsigned key[sample_candidates];
-        int index[sample_candidates];
-      };
-      mass_t hist256[256];      // on the row itself
-    };
+    unsigned key[sample_candidates];
+    int index[sample_candidates];
     union {
       mass_t hist[nt];
       int offsets[nt];
-      float table[128];
+      struct {
+        float most[sample_row_bins];  // upper bounds of mass
+        int count[sample_row_bins];
+      };
     };
     mass_t wave_mass[num_waves];
     double wave_sum[num_waves];
@@ -333,24 +350,40 @@ struct sample_row_f {
     int wave_int[num_waves];
     mass_t above, at;
     unsigned digit;
-    int count;
-    int picked;
+    int listed, picked;
+    int bracket[2];
     double rest;
   };
 
-  MGPU_DEVICE mass_t mass(unsigned key, float z_max, double c) const {
-    double e = key ? sample_exp2(((double)sample_value(key) -
-      (double)z_max) * c) : 0.;
-    return (mass_t)(e * (double)(1ull << scale) + .5);
+  // The row at hand, the same in all threads.
+  struct at_t {
+    int tid, row;
+    float m;                    // the largest logit
+    double u;
+    sample_row_t s;
+    const sample_piece_t* piece;
+    const type_t* z;
+  };
+
+  __forceinline__ MGPU_DEVICE double share(const at_t& a, float z) const {
+    return sample_exp2_t()(((double)z - (double)a.m) * a.s.c);
+  }
+  __forceinline__ MGPU_DEVICE mass_t whole(double share) const {
+    return (mass_t)(share * (double)(1ull << scale) + .5);
+  }
+  // What a kept token has after min-p.
+  __forceinline__ MGPU_DEVICE mass_t final_mass(const at_t& a, float z) const {
+    double e = share(a, z);
+    return e >= a.s.least || z == a.m ? whole(e) : 0;
   }
 
   // Keys without the bits below the type's own; +inf's, which has them, stays
   // above all others.
   enum : unsigned { top_key = 0xff7fffffu };
-  MGPU_DEVICE static unsigned rank_of(unsigned key) {
+  __forceinline__ MGPU_DEVICE static unsigned rank_of(unsigned key) {
     return (key + (key == top_key)) >> key_shift;
   }
-  MGPU_DEVICE static unsigned key_of(unsigned rank) {
+  __forceinline__ MGPU_DEVICE static unsigned key_of(unsigned rank) {
     if(rank == rank_of(top_key)) return top_key;
     unsigned key = rank << key_shift;
     // Negative logits have their bits inverted.
@@ -359,13 +392,13 @@ struct sample_row_f {
 
   // Folds that every thread may call again at once.
   template<typename t_t, typename op_t>
-  MGPU_DEVICE t_t fold(t_t x, op_t op, int tid, t_t (&shared)[num_waves]) const {
+  __forceinline__ MGPU_DEVICE t_t fold(t_t x, op_t op, int tid, t_t (&shared)[num_waves]) const {
     __syncthreads();
     return cta_allreduce<nt>(x, op, tid, shared);
   }
   // Inclusive scan over the CTA.
   template<typename t_t>
-  MGPU_DEVICE t_t scan(t_t x, int tid, t_t (&shared)[num_waves]) const {
+  __forceinline__ MGPU_DEVICE t_t scan(t_t x, int tid, t_t (&shared)[num_waves]) const {
     x = wave_scan(x, plus_t<t_t>(), tid & 63);
     __syncthreads();
     if(63 == (tid & 63)) shared[tid / 64] = x;
@@ -379,7 +412,7 @@ struct sample_row_f {
   // smallest value up to which, in ascending order, the weights sum up to
   // `want` (which their total reaches), the sum in front of it and its own.
   template<typename get_t>
-  MGPU_DEVICE unsigned select(int n, int bits, mass_t want, get_t get, int tid,
+  __forceinline__ MGPU_DEVICE unsigned select(int n, int bits, mass_t want, get_t get, int tid,
     shared_t& shared, mass_t& above, mass_t& at) const {
     unsigned prefix = 0;
     above = 0;
@@ -413,59 +446,80 @@ struct sample_row_f {
     return prefix;
   }
 
-  MGPU_DEVICE void done(int row, int v, float z_max, double c, double total) const {
-    float z = sample_clean((float)logits[row * stride + v]);
-    token[row] = v;
-    logprob[row] = (float)(((double)z - (double)z_max) * c *
+  __forceinline__ MGPU_DEVICE void done(const at_t& a, int v, double total) const {
+    float z = sample_clean((float)a.z[v]);
+    token[a.row] = v;
+    logprob[a.row] = (float)(((double)z - (double)a.m) * a.s.c *
       0.693147180559945309 - log(total));
   }
 
-  MGPU_DEVICE void operator()(int tid, int row) const {
+  __forceinline__ MGPU_DEVICE void operator()(int tid, int row) const {
     const float inf = __builtin_inff();
     __shared__ shared_t shared;
-    sample_row_t s = settings.row(row, vocab);
-    const sample_piece_t* piece = from + (int64_t)row * pieces;
-
+    at_t a;
+    a.tid = tid;
+    a.row = row;
+    a.piece = from + (int64_t)row * pieces;
+    a.z = logits + row * stride;
     float m = -inf;
-    for(int i = tid; i < pieces; i += nt) m = __builtin_fmaxf(m, piece[i].max);
-    m = fold(m, float_max_t(), tid, shared.wave_float);
-    if(m == -inf) {
+    for(int i = tid; i < pieces; i += nt) m = __builtin_fmaxf(m, a.piece[i].max);
+    a.m = fold(m, float_max_t(), tid, shared.wave_float);
+    if(a.m == -inf) {
       if(!tid) {
         token[row] = -1;
         logprob[row] = -inf;
       }
       return;
     }
+    a.s = settings.row(row, vocab);
     double u = uniform[row];
-    u = u > 0 ? __builtin_fmin(u, 1.) : 0;
+    a.u = u > 0 ? __builtin_fmin(u, 1.) : 0;
 
-    if(s.all()) { draw_from_all(tid, row, m, u, s, piece, shared); return; }
+    if(a.s.all()) { draw_from_all(a, shared); return; }
 
-    // The candidates.
-    int n;
+    // Nothing further down is drawn.
+    float reach = nothing_left();
+    if(a.s.least > 0)
+      reach = __builtin_fminf(reach, .01f - 2 * (float)log2(a.s.least));
     mass_t want = 0;
-    if(s.by_count) {
-      if(s.k > sample_max_k) { on_the_row(tid, row, m, u, s, 0, shared); return; }
-      n = gather_lists(tid, row, piece, shared);
+    double sum = 0;
+    int n = sample_candidates + 1;
+    bool counted = true;              // the tables by half octave are there
+    if(a.s.by_count && a.s.k <= sample_max_k) {
+      n = gather_lists(a, shared);
+      counted = false;
     } else {
-      float limit = 2.f * (scale + 2);
-      if(s.by_mass) limit = __builtin_fminf(limit, top_p_limit(tid, m, s, piece,
-        shared, want));
-      if(s.least > 0)
-        limit = __builtin_fminf(limit, .01f - 2 * (float)log2(s.least));
-      n = gather_row(tid, row, m, limit, s, shared);
+      if(a.s.by_count || a.s.by_mass) merge_tables(a, shared);
+      if(!a.s.by_count) {
+        float low, high = reach;
+        if(a.s.by_mass) {
+          sum = row_sum(a, shared);
+          want = goal(a.s.p * sum * (double)(1ull << scale));
+          bracket_mass(a, sum, low, high, shared);
+          high = __builtin_fminf(high, reach);
+        }
+        n = list_down_to(a, high, shared);
+      }
     }
-    if(n > sample_candidates) { on_the_row(tid, row, m, u, s, want, shared); return; }
-    on_the_list(tid, row, m, u, s, n, want, shared);
+    if(n <= sample_candidates) on_the_list(a, n, want, shared);
+    else on_the_row(a, reach, want, sum, counted, shared);
+  }
+
+  // Half octaves below the largest logit at which no probability is left.
+  __forceinline__ MGPU_DEVICE float nothing_left() const { return 2.f * (scale + 2); }
+
+  // Kept are those in front of whom there is less than x, a whole number
+  // below its ceiling; the first always.
+  __forceinline__ MGPU_DEVICE static mass_t goal(double x) {
+    return max((mass_t)ceil(x), (mass_t)1);
   }
 
   // The pieces' lists, one after the other.
-  MGPU_DEVICE int gather_lists(int tid, int row, const sample_piece_t* piece,
-    shared_t& shared) const {
-    int base = 0;
+  __forceinline__ MGPU_DEVICE int gather_lists(const at_t& a, shared_t& shared) const {
+    int base = 0, tid = a.tid;
     bool too_many = false;
     for(int p0 = 0; p0 < pieces; p0 += nt) {
-      int mine = p0 + tid < pieces ? piece[p0 + tid].listed : 0;
+      int mine = p0 + tid < pieces ? a.piece[p0 + tid].listed : 0;
       too_many |= mine > sample_list;
       int upto = scan(min(mine, (int)sample_list), tid, shared.wave_int);
       __syncthreads();
@@ -477,10 +531,9 @@ struct sample_row_f {
         int first = p ? shared.offsets[p - 1] : 0;
         int count = shared.offsets[p] - first;
         for(int i = tid & 63; i < count; i += 64) {
-          int v = (p0 + p) * sample_piece + piece[p0 + p].list[i];
+          int v = (p0 + p) * sample_piece + a.piece[p0 + p].list[i];
           shared.index[base + first + i] = v;
-          shared.key[base + first + i] =
-            sample_key((float)logits[row * stride + v]);
+          shared.key[base + first + i] = sample_key((float)a.z[v]);
         }
       }
       base += shared.offsets[here - 1];
@@ -489,179 +542,474 @@ struct sample_row_f {
     return base;
   }
 
-  // The row's tokens whose logits lie within `limit` half octaves of the
-  // largest.
-  MGPU_DEVICE int gather_row(int tid, int row, float m, float limit,
-    const sample_row_t& s, shared_t& shared) const {
-    enum { unroll = 32 / W };
-    const type_t* z = logits + row * stride;
-    if(!tid) shared.count = 0;
-    __syncthreads();
-    for(int v0 = tid * W; v0 - tid * W < vocab; v0 += nt * W * unroll) {
+  // use(v, chunks): 16 tokens of every thread at a time; chunk c begins at
+  // token v + c * nt * W.
+  template<typename use_t>
+  __forceinline__ MGPU_DEVICE void sweep(const at_t& a, use_t use) const {
+    for(int v0 = 0; v0 < vocab; v0 += nt * W * unroll) {
+      int v = v0 + a.tid * W;
       row_chunk_t<type_t> ch[unroll];
       PRAGMA_UNROLL
       for(int c = 0; c < unroll; ++c)
-        ch[c].load(z + v0 + c * nt * W, vocab - v0 - c * nt * W,
+        ch[c].load(a.z + v + c * nt * W, vocab - v - c * nt * W,
           (type_t)-__builtin_inff());
+      use(v, ch);
+    }
+  }
+
+  // The row's tokens by half octaves below its largest logit.
+  __forceinline__ MGPU_DEVICE void clear_tables(const at_t& a, shared_t& shared) const {
+    __syncthreads();
+    if(a.tid < sample_row_bins) {
+      shared.most[a.tid] = 0;
+      shared.count[a.tid] = 0;
+    }
+    __syncthreads();
+  }
+  // From the pieces' tables, shifted down to the row's largest logit: bin b
+  // has the tokens of b - 2 to b below it, the last one all the others.
+  __forceinline__ MGPU_DEVICE void merge_tables(const at_t& a, shared_t& shared) const {
+    clear_tables(a, shared);
+    for(int i = a.tid; i < pieces * sample_bins; i += nt) {
+      const sample_piece_t& from = a.piece[i / sample_bins];
+      int bin = i % sample_bins, n = 0;
+      float off = (a.m - from.max) * a.s.c2;
+      if(off < sample_row_bins) n = from.table[bin];
+      if(n) {
+        int to = sample_bins - 1 == bin ? sample_row_bins - 1 :
+          min((int)ceilf(off) + bin + 1, sample_row_bins - 1);
+        atomicAdd(&shared.most[to],
+          n * __builtin_amdgcn_exp2f(-.5f * (off + bin)));
+        atomicAdd(&shared.count[to], n);
+      }
+    }
+    __syncthreads();
+  }
+  // From the row.
+  __forceinline__ MGPU_DEVICE void count_row(const at_t& a, shared_t& shared) const {
+    clear_tables(a, shared);
+    sweep(a, [&](int, const row_chunk_t<type_t> (&ch)[unroll]) {
+      PRAGMA_UNROLL
+      for(int i = 0; i < per_thread; ++i) {
+        float x = sample_clean((float)ch[i / W].x[i % W]);
+        if(x > -__builtin_inff())
+          atomicAdd(&shared.count[1 + (int)__builtin_fminf((a.m - x) * a.s.c2,
+            sample_row_bins - 2)], 1);
+      }
+    });
+    __syncthreads();
+    if(a.tid < sample_row_bins)
+      shared.most[a.tid] = shared.count[a.tid] *
+        __builtin_amdgcn_exp2f(-.5f * (a.tid - 1));
+    __syncthreads();
+  }
+
+  // Brackets, in half octaves below the largest logit: every token less than
+  // `low` down is above the border, none more than `high` down is.
+  __forceinline__ MGPU_DEVICE void store_bracket(const at_t& a, int before, int last,
+    float& low, float& high, shared_t& shared) const {
+    // `before` bins are in front of the border, and hold every token down to
+    // before - 3 (a piece's tokens past its 63rd bin are in the last bin); the
+    // border is in bin `last` at most.
+    if(!a.tid) {
+      shared.bracket[0] = min(before - 3, sample_bins - 2);
+      shared.bracket[1] = last;
+    }
+    __syncthreads();
+    low = shared.bracket[0];
+    high = shared.bracket[1] >= sample_row_bins - 2 ? __builtin_inff() :
+      shared.bracket[1] + .01f;
+    __syncthreads();
+  }
+  __forceinline__ MGPU_DEVICE void bracket(const at_t& a, bool by_mass,
+    double sum, float& low, float& high, shared_t& shared) const {
+    if(by_mass) bracket_mass(a, sum, low, high, shared);
+    else bracket_count(a, low, high, shared);
+  }
+  __forceinline__ MGPU_DEVICE void bracket_count(const at_t& a, float& low, float& high,
+    shared_t& shared) const {
+    int less = 0;
+    if(a.tid < 64) {
+      int x = shared.count[2 * a.tid], y = shared.count[2 * a.tid + 1];
+      int upto = wave_scan(x + y, plus_t<int>(), a.tid);
+      less = popc(ballot(upto - y < a.s.k)) + popc(ballot(upto < a.s.k));
+    }
+    store_bracket(a, less, less, low, high, shared);
+  }
+  // Sums of 32-bit floats of up to 64 * pieces terms are off by 4e-6 * pieces
+  // at most.
+  __forceinline__ MGPU_DEVICE void bracket_mass(const at_t& a, double sum, float& low,
+    float& high, shared_t& shared) const {
+    int before = 0, last = 0;
+    if(a.tid < 64) {
+      float margin = 1.0001f + 1e-5f * pieces;
+      float x = shared.most[2 * a.tid], y = shared.most[2 * a.tid + 1];
+      float upto = wave_scan(x + y, plus_t<float>(), a.tid);
+      float want = (float)(a.s.p * sum) / margin;
+      before = popc(ballot(upto - y < want)) + popc(ballot(upto < want));
+      // Bins with more than 1 - p from them on.
+      x = shared.most[127 - 2 * a.tid], y = shared.most[126 - 2 * a.tid];
+      upto = wave_scan(x + y, plus_t<float>(), a.tid);
+      float rest = (float)((1 - a.s.p) * sum) / margin;
+      last = popc(ballot(upto - y > rest)) + popc(ballot(upto > rest)) - 1;
+    }
+    store_bracket(a, before, last, low, high, shared);
+  }
+
+  // The row's sum of 2^((z - m) c).
+  __forceinline__ MGPU_DEVICE double row_sum(const at_t& a, shared_t& shared) const {
+    double sum = 0;
+    for(int i = a.tid; i < pieces; i += nt)
+      if(a.piece[i].max > -__builtin_inff())
+        sum += a.piece[i].sum *
+          sample_exp2_t()(((double)a.piece[i].max - (double)a.m) * a.s.c);
+    return fold(sum, plus_t<double>(), a.tid, shared.wave_sum);
+  }
+
+  // Adds the tokens with a bit set to the list.
+  __forceinline__ MGPU_DEVICE void append(const at_t& a, int v,
+    const row_chunk_t<type_t> (&ch)[unroll], unsigned in, shared_t& shared)
+    const {
+    int n = popc(in);
+    int at = wave_scan(n, plus_t<int>(), a.tid & 63);
+    int base = 0;
+    if(63 == (a.tid & 63) && at) base = atomicAdd(&shared.listed, at);
+    at += readlane(base, 63) - n;
+    PRAGMA_UNROLL
+    for(int i = 0; i < per_thread; ++i)
+      if(in >> i & 1) {
+        if(at < sample_candidates) {
+          shared.key[at] = sample_key((float)ch[i / W].x[i % W]);
+          shared.index[at] = v + i / W * nt * W + i % W;
+        }
+        ++at;
+      }
+  }
+
+  // Lists the tokens down to `high` half octaves below the largest logit and
+  // returns how many there are; more than sample_candidates: not all listed.
+  __forceinline__ MGPU_DEVICE int list_down_to(const at_t& a, float high,
+    shared_t& shared) const {
+    __syncthreads();
+    if(!a.tid) shared.listed = 0;
+    __syncthreads();
+    sweep(a, [&](int v, const row_chunk_t<type_t> (&ch)[unroll]) {
       unsigned in = 0;
       PRAGMA_UNROLL
-      for(int i = 0; i < 32; ++i) {
+      for(int i = 0; i < per_thread; ++i) {
         float x = sample_clean((float)ch[i / W].x[i % W]);
-        if(x > -__builtin_inff() && (m - x) * s.c2 <= limit) in |= 1u << i;
+        // (NaN, for a difference past the largest float at c2 = 0, is in)
+        if(x > -__builtin_inff() && !((a.m - x) * a.s.c2 > high)) in |= 1u << i;
       }
-      int n = popc(in);
-      int at = wave_scan(n, plus_t<int>(), tid & 63);
-      int base = 0;
-      if(63 == (tid & 63) && at) base = atomicAdd(&shared.count, at);
-      at += readlane(base, 63) - n;
+      append(a, v, ch, in, shared);
+    });
+    __syncthreads();
+    return shared.listed;
+  }
+
+  // The same within the cut, without the tokens less than `low` down: those are
+  // added up (counted, or their mass).
+  __forceinline__ MGPU_DEVICE mass_t add_above(const at_t& a, bool by_mass,
+    sample_cut_t cut, float low, float high, int& listed, shared_t& shared)
+    const {
+    __syncthreads();
+    if(!a.tid) shared.listed = 0;
+    __syncthreads();
+    mass_t sum = 0;
+    sweep(a, [&](int v, const row_chunk_t<type_t> (&ch)[unroll]) {
+      unsigned in = 0;
       PRAGMA_UNROLL
-      for(int i = 0; i < 32; ++i)
-        if(in >> i & 1) {
-          if(at < sample_candidates) {
-            shared.key[at] = sample_key((float)ch[i / W].x[i % W]);
-            shared.index[at] = v0 + i / W * nt * W + i % W;
-          }
-          ++at;
+      for(int i = 0; i < per_thread; ++i) {
+        float x = sample_clean((float)ch[i / W].x[i % W]);
+        float down = (a.m - x) * a.s.c2;
+        if(x > -__builtin_inff() && !(down > high) &&
+          cut.keeps(sample_key(x), v + i / W * nt * W + i % W)) {
+          if(!(down < low)) in |= 1u << i;
+          else sum += by_mass ? whole(share(a, x)) : 1;
         }
-    }
-    __syncthreads();
-    return shared.count;
-  }
-
-  // top-p without top-k: the mass that has to be reached, and how many half
-  // octaves below the largest logit it is reached for sure.
-  MGPU_DEVICE float top_p_limit(int tid, float m, const sample_row_t& s,
-    const sample_piece_t* piece, shared_t& shared, mass_t& want) const {
-    double sum = 0;
-    for(int i = tid; i < pieces; i += nt)
-      if(piece[i].max > -__builtin_inff())
-        sum += piece[i].sum *
-          sample_exp2(((double)piece[i].max - (double)m) * s.c);
-    sum = fold(sum, plus_t<double>(), tid, shared.wave_sum);
-    want = max((mass_t)ceil(s.p * sum * (double)(1ull << scale)), (mass_t)1);
-
-    // The pieces' tables, shifted down to the row's largest logit and
-    // rounded down to whole half octaves.
-    if(tid < 128) shared.table[tid] = 0;
-    __syncthreads();
-    for(int i = tid; i < pieces * sample_bins; i += nt) {
-      const sample_piece_t& from = piece[i / sample_bins];
-      int bin = i % sample_bins;
-      float off = (m - from.max) * s.c2;
-      if(off < 64) {
-        float x = from.table[bin] * __builtin_amdgcn_exp2f(-.5f * off);
-        int to = sample_bins - 1 == bin ? 127 : min((int)ceilf(off) + bin + 1, 127);
-        if(x > 0) atomicAdd(&shared.table[to], x);
       }
-    }
-    __syncthreads();
-    if(tid < 64) {
-      // 32-bit sums of up to 64 * pieces terms: off by 4e-6 * pieces at most.
-      float goal = (float)(s.p * sum) * (1.0001f + 1e-5f * pieces);
-      float a = shared.table[2 * tid], b = shared.table[2 * tid + 1];
-      float upto = wave_scan(a + b, plus_t<float>(), tid);
-      lanemask_t enough = ballot(upto >= goal);
-      if(!tid) shared.count = enough ? 2 * ffs(enough) - 1 : 127;
-    }
-    __syncthreads();
-    int cut = shared.count;
-    __syncthreads();
-    return cut >= 126 ? __builtin_inff() : cut + .01f;
+      append(a, v, ch, in, shared);
+    });
+    sum = fold(sum, plus_t<mass_t>(), a.tid, shared.wave_mass);
+    listed = shared.listed;
+    return sum;
   }
 
-  // A list of n candidates that holds every token to be kept.
-  MGPU_DEVICE void on_the_list(int tid, int row, float m, double u,
-    const sample_row_t& s, int n, mass_t want, shared_t& shared) const {
-    __syncthreads();
-    unsigned best = rank_of(sample_key(m));
+  // The border among n listed tokens, of which those within `cut` count: kept
+  // are the ones in front of whom there is less than `want`, which they reach
+  // together.
+  __forceinline__ MGPU_DEVICE sample_cut_t border_of(const at_t& a, int n, bool by_mass,
+    sample_cut_t cut, mass_t want, shared_t& shared) const {
+    unsigned best = rank_of(sample_key(a.m));
     auto down = [&](int i) { return best - rank_of(shared.key[i]); };
     unsigned deepest = 0;
-    for(int i = tid; i < n; i += nt) deepest = max(deepest, down(i));
-    deepest = fold(deepest, maximum_t<unsigned>(), tid,
+    for(int i = a.tid; i < n; i += nt) deepest = max(deepest, down(i));
+    deepest = fold(deepest, maximum_t<unsigned>(), a.tid,
       (unsigned (&)[num_waves])shared.wave_int);
-    int bits = 32 - clz(deepest);
-    int index_bits = 32 - clz((unsigned)vocab - 1);
     mass_t above, at;
-
-    // Kept: those above the border, and of those on it the ones up to last.
-    unsigned border = deepest;
-    int last = vocab;
-    auto kept = [&](int i, unsigned& d) {
-      d = down(i);
-      return d < border || (d == border && shared.index[i] <= last);
-    };
-    auto cut_ties = [&](mass_t ties) {
-      last = (int)select(n, index_bits, ties,
+    unsigned to = select(n, 32 - clz(deepest), want,
+      [&](int i, unsigned& value, mass_t& weight) {
+        if(!cut.keeps(shared.key[i], shared.index[i])) return false;
+        value = down(i);
+        weight = by_mass ? whole(share(a, sample_value(shared.key[i]))) : 1;
+        return true;
+      }, a.tid, shared, above, at);
+    sample_cut_t found = { key_of(best - to), vocab };
+    mass_t each = by_mass ? whole(share(a, sample_value(found.key))) : 1;
+    mass_t ties = (want - above + each - 1) / each;
+    if(found.key == cut.key) found.last = cut.last;
+    if(ties * each < at) {
+      sample_cut_t ends = found;
+      found.last = (int)select(n, 32 - clz((unsigned)vocab - 1), ties,
         [&](int i, unsigned& value, mass_t& weight) {
-          unsigned d;
           value = shared.index[i];
           weight = 1;
-          return kept(i, d) && d == border;
-        }, tid, shared, above, at);
-    };
+          return shared.key[i] == ends.key && (int)value <= ends.last;
+        }, a.tid, shared, above, at);
+    }
+    return found;
+  }
 
-    if(s.by_count && n > s.k) {
-      border = select(n, bits, s.k,
-        [&](int i, unsigned& value, mass_t& weight) {
-          value = down(i);
-          weight = 1;
-          return true;
-        }, tid, shared, above, at);
-      mass_t ties = s.k - above;
-      if(ties < at) cut_ties(ties);
-    }
-    if(s.by_mass) {
-      mass_t all = 0;
-      for(int i = tid; i < n; i += nt) {
-        unsigned d;
-        if(kept(i, d)) all += mass(shared.key[i], m, s.c);
+  __forceinline__ MGPU_DEVICE mass_t mass_within(const at_t& a, int n,
+    sample_cut_t cut, shared_t& shared) const {
+    mass_t all = 0;
+    for(int i = a.tid; i < n; i += nt)
+      if(cut.keeps(shared.key[i], shared.index[i]))
+        all += whole(share(a, sample_value(shared.key[i])));
+    return fold(all, plus_t<mass_t>(), a.tid, shared.wave_mass);
+  }
+
+  // n candidates that hold every token to be kept.  want: top-p's without
+  // top-k.
+  __forceinline__ MGPU_DEVICE void on_the_list(const at_t& a, int n, mass_t want,
+    shared_t& shared) const {
+    __syncthreads();
+    sample_cut_t cut = { 0, vocab };
+    PRAGMA_NO_UNROLL
+    for(int by_mass = 0; by_mass < 2; ++by_mass) {
+      if(by_mass ? !a.s.by_mass : !a.s.by_count) continue;
+      mass_t all = n;
+      if(by_mass) {
+        all = mass_within(a, n, cut, shared);
+        if(a.s.by_count) want = goal(a.s.p * (double)all);
       }
-      all = fold(all, plus_t<mass_t>(), tid, shared.wave_mass);
-      if(s.by_count)
-        want = max((mass_t)ceil(s.p * (double)all), (mass_t)1);
-      if(want <= all) {
-        unsigned to = select(n, bits, want,
-          [&](int i, unsigned& value, mass_t& weight) {
-            if(!kept(i, value)) return false;
-            weight = mass(shared.key[i], m, s.c);
-            return true;
-          }, tid, shared, above, at);
-        mass_t each = mass(key_of(best - to), m, s.c);
-        mass_t ties = (want - above + each - 1) / each;
-        if(to != border) last = vocab;
-        border = to;
-        if(ties * each < at) cut_ties(ties);
-      }
+      mass_t need = by_mass ? want : (mass_t)a.s.k;
+      if(need < all) cut = border_of(a, n, by_mass, cut, need, shared);
     }
-    auto final_mass = [&](int i) -> mass_t {
-      unsigned d;
-      if(!kept(i, d)) return 0;
-      double e = sample_exp2(((double)sample_value(shared.key[i]) -
-        (double)m) * s.c);
-      return !d || e >= s.least ?
-        (mass_t)(e * (double)(1ull << scale) + .5) : 0;
+    auto mass = [&](int i) -> mass_t {
+      return cut.keeps(shared.key[i], shared.index[i]) ?
+        final_mass(a, sample_value(shared.key[i])) : 0;
     };
     mass_t total = 0;
-    for(int i = tid; i < n; i += nt) total += final_mass(i);
-    total = fold(total, plus_t<mass_t>(), tid, shared.wave_mass);
-    mass_t target = min((mass_t)(u * (double)total), total - 1);
-    int v = (int)select(n, index_bits, target + 1,
+    for(int i = a.tid; i < n; i += nt) total += mass(i);
+    total = fold(total, plus_t<mass_t>(), a.tid, shared.wave_mass);
+    mass_t target = min((mass_t)(a.u * (double)total), total - 1), above, at;
+    int v = (int)select(n, 32 - clz((unsigned)vocab - 1), target + 1,
       [&](int i, unsigned& value, mass_t& weight) {
         value = shared.index[i];
-        weight = final_mass(i);
+        weight = mass(i);
         return weight > 0;
-      }, tid, shared, above, at);
-    if(!tid) done(row, v, m, s.c, (double)total / (double)(1ull << scale));
+      }, a.tid, shared, above, at);
+    if(!a.tid) done(a, v, (double)total / (double)(1ull << scale));
+  }
+
+  // Too many for the list: one reading of the row per border (and one for the
+  // total between top-k and top-p), and one for the draw.  want, sum: top-p's
+  // without top-k.
+  __forceinline__ MGPU_DEVICE void on_the_row(const at_t& a, float reach,
+    mass_t want, double sum, bool counted, shared_t& shared) const {
+    enum { border_by_count, total, border_by_mass };
+    sample_cut_t cut = { 0, vocab };
+    PRAGMA_NO_UNROLL
+    for(int step = border_by_count; step <= border_by_mass; ++step) {
+      bool by_mass = step != border_by_count;
+      if((step <= total && !a.s.by_count) || (by_mass && !a.s.by_mass))
+        continue;
+      float low = __builtin_inff(), high = nothing_left();
+      if(step != total) {
+        if(!counted) {
+          count_row(a, shared);
+          counted = true;
+        }
+        float down;
+        bracket(a, by_mass, sum, low, down, shared);
+        high = __builtin_fminf(high, down);
+      }
+      int n;
+      mass_t above = add_above(a, by_mass, cut, low, high, n, shared);
+      if(step == total) {
+        want = goal(a.s.p * (double)above);
+        sum = (double)above / (double)(1ull << scale);
+        continue;
+      }
+      mass_t need = by_mass ? want : (mass_t)a.s.k;
+      if(n > sample_candidates) {
+        cut = border_on_row(a, by_mass, cut, need, shared);
+        counted = false;                      // hist lies over the tables
+      } else {
+        mass_t all = above + (by_mass ? mass_within(a, n, cut, shared) :
+          (mass_t)n);
+        if(need < all) {
+          cut = border_of(a, n, by_mass, cut, need - above, shared);
+          counted = false;
+        }
+      }
+    }
+    draw_on_row(a, cut, reach, shared);
+  }
+
+  // The border by 8 bits of the key at a time: more tokens than fit the list
+  // lie within the bracket (many equal ones, or a temperature at which all
+  // are).
+  __forceinline__ MGPU_DEVICE sample_cut_t border_on_row(const at_t& a, bool by_mass,
+    sample_cut_t cut, mass_t want, shared_t& shared) const {
+    unsigned prefix = 0;
+    mass_t above = 0, at = 0;
+    PRAGMA_NO_UNROLL
+    for(int shift = 24; shift >= 0; shift -= 8) {
+      __syncthreads();
+      if(a.tid < 256) shared.hist[a.tid] = 0;
+      if(!a.tid) shared.picked = -1;
+      __syncthreads();
+      unsigned high = shift == 24 ? 0u : ~0u << (shift + 8);
+      sweep(a, [&](int v, const row_chunk_t<type_t> (&ch)[unroll]) {
+        PRAGMA_UNROLL
+        for(int i = 0; i < per_thread; ++i) {
+          float x = sample_clean((float)ch[i / W].x[i % W]);
+          unsigned key = sample_key(x);
+          if(key && (key & high) == prefix &&
+            cut.keeps(key, v + i / W * nt * W + i % W))
+            atomicAdd(&shared.hist[(key >> shift) & 255],
+              by_mass ? whole(share(a, x)) : (mass_t)1);
+        }
+      });
+      __syncthreads();
+      // The digit at which the sum from the top reaches `want`.
+      mass_t mine = a.tid < 256 ? shared.hist[255 - a.tid] : 0;
+      mass_t upto = above + scan(mine, a.tid, shared.wave_mass);
+      if(upto - mine < want && want <= upto) {
+        shared.picked = 255 - a.tid;
+        shared.above = upto - mine;
+        shared.at = mine;
+      }
+      __syncthreads();
+      if(shared.picked < 0) return cut;           // not reached: all are kept
+      prefix |= (unsigned)shared.picked << shift;
+      above = shared.above;
+      at = shared.at;
+    }
+    sample_cut_t found = { prefix, prefix == cut.key ? cut.last : vocab };
+    mass_t each = by_mass ? whole(share(a, sample_value(prefix))) : 1;
+    mass_t ties = (want - above + each - 1) / each;
+    if(ties * each >= at) return found;
+    // The index of the last of the ties, by its digits.
+    unsigned last = 0;
+    mass_t before = 0;
+    PRAGMA_NO_UNROLL
+    for(int left = 24; left > 0; left -= 8) {
+      int shift = left - 8;
+      __syncthreads();
+      if(a.tid < 256) shared.hist[a.tid] = 0;
+      __syncthreads();
+      sweep(a, [&](int v, const row_chunk_t<type_t> (&ch)[unroll]) {
+        PRAGMA_UNROLL
+        for(int i = 0; i < per_thread; ++i) {
+          unsigned at = v + i / W * nt * W + i % W;
+          if((int)at < vocab && at >> left == last >> left &&
+            (int)at <= found.last &&
+            sample_key(sample_clean((float)ch[i / W].x[i % W])) == prefix)
+            atomicAdd(&shared.hist[(at >> shift) & 255], (mass_t)1);
+        }
+      });
+      __syncthreads();
+      mass_t mine = a.tid < 256 ? shared.hist[a.tid] : 0;
+      mass_t upto = before + scan(mine, a.tid, shared.wave_mass);
+      if(upto - mine < ties && ties <= upto) {
+        shared.digit = a.tid;
+        shared.above = upto - mine;
+      }
+      __syncthreads();
+      last |= shared.digit << shift;
+      before = shared.above;
+    }
+    found.last = (int)last;
+    return found;
+  }
+
+  // The draw from the row's tokens within the cut: their mass by runs of
+  // 64 * W tokens (or a power of two of those), the run that holds the target,
+  // the token.
+  __forceinline__ MGPU_DEVICE void draw_on_row(const at_t& a, sample_cut_t cut, float reach,
+    shared_t& shared) const {
+    enum { run = 64 * W };
+    int tid = a.tid, more = 0;
+    while((vocab - 1) / run >> more >= nt) ++more;
+    auto mass = [&](float x, int v) -> mass_t {
+      return x > -__builtin_inff() && !((a.m - x) * a.s.c2 > reach) &&
+        (!cut.key || cut.keeps(sample_key(x), v)) ? final_mass(a, x) : 0;
+    };
+    __syncthreads();
+    shared.hist[tid] = 0;
+    __syncthreads();
+    sweep(a, [&](int v, const row_chunk_t<type_t> (&ch)[unroll]) {
+      PRAGMA_UNROLL
+      for(int c = 0; c < unroll; ++c) {
+        mass_t sum = 0;
+        int v0 = v + c * nt * W;
+        PRAGMA_UNROLL
+        for(int i = 0; i < W; ++i)
+          sum += mass(sample_clean((float)ch[c].x[i]), v0 + i);
+        sum = wave_allreduce(sum, plus_t<mass_t>(), tid & 63);
+        if(!(tid & 63) && sum)
+          atomicAdd(&shared.hist[v0 / run >> more], sum);
+      }
+    });
+    __syncthreads();
+    mass_t mine = shared.hist[tid];
+    mass_t upto = scan(mine, tid, shared.wave_mass);
+    mass_t total = fold(mine, plus_t<mass_t>(), tid, shared.wave_mass);
+    mass_t target = min((mass_t)(a.u * (double)total), total - 1);
+    if(upto - mine <= target && target < upto) {
+      shared.picked = tid;
+      shared.above = upto - mine;
+    }
+    __syncthreads();
+    if(tid >= 64) return;
+    mass_t rest = target - shared.above;
+    int first = (shared.picked << more) * run, end = vocab;
+    for(int v0 = first; v0 < end; v0 += run) {
+      int v = v0 + tid * W;
+      row_chunk_t<type_t> ch;
+      ch.load(a.z + v, vocab - v, (type_t)-__builtin_inff());
+      mass_t x[W], sum = 0;
+      PRAGMA_UNROLL
+      for(int i = 0; i < W; ++i)
+        sum += x[i] = mass(sample_clean((float)ch.x[i]), v + i);
+      mass_t to = wave_scan(sum, plus_t<mass_t>(), tid);
+      mass_t all = readlane(to, 63);
+      if(rest < all) {
+        to -= sum;
+        PRAGMA_UNROLL
+        for(int i = 0; i < W; ++i) {
+          if(to <= rest && rest < to + x[i])
+            done(a, v + i, (double)total / (double)(1ull << scale));
+          to += x[i];
+        }
+        return;
+      }
+      rest -= all;
+    }
   }
 
   // Every token counts: the piece, the run of tokens in it, and the token at
   // which the running sum passes u times the total.
-  MGPU_DEVICE void draw_from_all(int tid, int row, float m, double u,
-    const sample_row_t& s, const sample_piece_t* piece, shared_t& shared) const {
+  __forceinline__ MGPU_DEVICE void draw_from_all(const at_t& a, shared_t& shared) const {
+    int tid = a.tid;
     double before = 0, total = 0;
     auto scaled = [&](int p) {
-      return p < pieces && piece[p].max > -__builtin_inff() ? piece[p].sum *
-        sample_exp2(((double)piece[p].max - (double)m) * s.c) : 0.;
+      return p < pieces && a.piece[p].max > -__builtin_inff() ?
+        a.piece[p].sum *
+          sample_exp2_t()(((double)a.piece[p].max - (double)a.m) * a.s.c) : 0.;
     };
     for(int p0 = 0; p0 < pieces; p0 += nt) {
       double upto = scan(scaled(p0 + tid), tid, shared.wave_sum);
@@ -670,7 +1018,7 @@ struct sample_row_f {
       total += shared.rest;
       __syncthreads();
     }
-    double target = u * total;
+    double target = a.u * total;
     if(!tid) shared.picked = -1;
     for(int p0 = 0; p0 < pieces; p0 += nt) {
       double x = scaled(p0 + tid);
@@ -681,10 +1029,10 @@ struct sample_row_f {
         (unsigned)(p0 + tid));
       __syncthreads();
       if(p0 + tid == shared.picked) shared.rest = target - (upto - x);
-      if(nt - 1 == tid) shared.above = (mass_t)__builtin_bit_cast(long long, upto);
+      if(nt - 1 == tid) shared.wave_sum[0] = upto;
       __syncthreads();
       if(shared.picked >= 0) break;
-      before = __builtin_bit_cast(double, (long long)shared.above);
+      before = shared.wave_sum[0];
       __syncthreads();
     }
     if(tid >= 64) return;
@@ -694,10 +1042,11 @@ struct sample_row_f {
       for(p = pieces - 1; !(scaled(p) > 0); --p);
       rest = __builtin_inf();
     }
-    double up = sample_exp2(((double)piece[p].max - (double)m) * s.c);
-    rest = rest / up;                   // in the piece's own measure
+    float m = a.piece[p].max;
+    // in the piece's own measure
+    rest = rest / sample_exp2_t()(((double)m - (double)a.m) * a.s.c);
     const int segments = sample_segments / (W / 4);
-    double x = tid < segments ? piece[p].segments[tid] : 0.;
+    double x = tid < segments ? a.piece[p].segments[tid] : 0.;
     double upto = wave_scan(x, plus_t<double>(), tid);
     lanemask_t past = ballot(x > 0 && upto > rest), any = ballot(x > 0);
     int segment = past ? ffs(past) - 1 : 63 - clz(any);
@@ -705,14 +1054,12 @@ struct sample_row_f {
     // Its 64 chunks of W tokens.
     int v0 = p * sample_piece + (segment * 64 + tid) * W;
     row_chunk_t<type_t> ch;
-    ch.load(logits + row * stride + v0, vocab - v0, (type_t)-__builtin_inff());
+    ch.load(a.z + v0, vocab - v0, (type_t)-__builtin_inff());
     double e[W];
     x = 0;
     PRAGMA_UNROLL
     for(int i = 0; i < W; ++i) {
-      float z = sample_clean((float)ch.x[i]);
-      e[i] = z > -__builtin_inff() ? sample_exp2(((double)z -
-        (double)piece[p].max) * s.c) : 0.;
+      e[i] = sample_exp2_t()(((double)sample_clean((float)ch.x[i]) - (double)m) * a.s.c);
       x += e[i];
     }
     upto = wave_scan(x, plus_t<double>(), tid);
@@ -727,100 +1074,7 @@ struct sample_row_f {
         sum += e[i];
         if(!found && e[i] > 0) { v = v0 + i; found = past && sum > rest; }
       }
-      done(row, v, m, s.c, total);
-    }
-  }
-
-  // On the row itself, by 8 bits of the key at a time: for k past
-  // sample_max_k, and where more than sample_candidates tokens qualify.
-  MGPU_DEVICE void on_the_row(int tid, int row, float m, double u,
-    const sample_row_t& s, mass_t want_mass, shared_t& shared) const {
-    const type_t* z = logits + row * stride;
-    unsigned best = sample_key(m);
-    unsigned border = 1;              // keys above it are kept,
-    mass_t ties = vocab;              // and so many that equal it
-    PRAGMA_UNROLL
-    for(int by_mass = 0; by_mass < 2; ++by_mass) {
-      if(by_mass ? !s.by_mass : !s.by_count) continue;
-      mass_t want = by_mass ? want_mass : (mass_t)s.k;
-      if(by_mass && s.by_count) {
-        mass_t all = 0, equal = 0;
-        for(int v = tid; v < vocab; v += nt) {
-          unsigned key = sample_key((float)z[v]);
-          if(key > border) all += mass(key, m, s.c);
-          else if(key == border) ++equal;
-        }
-        all = fold(all, plus_t<mass_t>(), tid, shared.wave_mass);
-        equal = fold(equal, plus_t<mass_t>(), tid, shared.wave_mass);
-        all += min(equal, ties) * mass(border, m, s.c);
-        want = max((mass_t)ceil(s.p * (double)all), (mass_t)1);
-      }
-      unsigned prefix = 0;
-      mass_t above = 0;               // count or mass of the keys above
-      for(int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if(tid < 256) shared.hist256[tid] = 0;
-        __syncthreads();
-        unsigned high = shift == 24 ? 0u : ~0u << (shift + 8);
-        for(int v = tid; v < vocab; v += nt) {
-          unsigned key = sample_key((float)z[v]);
-          if((key & high) == prefix && key >= border)
-            atomicAdd(&shared.hist256[(key >> shift) & 255],
-              by_mass ? mass(key, m, s.c) : (mass_t)1);
-        }
-        __syncthreads();
-        // The digit at which the sum from the top reaches `want`.
-        if(!tid) {
-          mass_t sum = above;
-          int d = 255;
-          for(; d > 0 && sum + shared.hist256[d] < want; --d)
-            sum += shared.hist256[d];
-          shared.digit = d;
-          shared.above = sum;
-        }
-        __syncthreads();
-        prefix |= shared.digit << shift;
-        above = shared.above;
-      }
-      mass_t each = by_mass ? mass(prefix, m, s.c) : (mass_t)1;
-      mass_t fit = each ? (want - above + each - 1) / each : (mass_t)0;
-      if(prefix > border) { border = prefix; ties = fit; }
-      else if(prefix == border) ties = min(ties, fit);
-    }
-
-    // The kept mass: one contiguous piece of the row per thread.
-    int piece = div_up(vocab, (int)nt);
-    int begin = min(tid * piece, vocab), end = min(begin + piece, vocab);
-    int equal = 0;
-    for(int v = begin; v < end; ++v)
-      equal += sample_key((float)z[v]) == border;
-    int before = scan(equal, tid, shared.wave_int) - equal;
-    auto kept = [&](int v, int& rank) -> mass_t {
-      unsigned key = sample_key((float)z[v]);
-      bool in = key > border;
-      if(key == border) in = (mass_t)rank++ < ties;
-      if(!in || !key) return 0;
-      double e = sample_exp2(((double)sample_value(key) - (double)m) * s.c);
-      return e >= s.least || key == best ?
-        (mass_t)(e * (double)(1ull << scale) + .5) : 0;
-    };
-    int rank = before;
-    mass_t mine = 0;
-    for(int v = begin; v < end; ++v) mine += kept(v, rank);
-    mass_t upto = scan(mine, tid, shared.wave_mass);
-    mass_t total = fold(mine, plus_t<mass_t>(), tid, shared.wave_mass);
-
-    mass_t target = min((mass_t)(u * (double)total), total - 1);
-    mass_t sum = upto - mine;
-    if(sum <= target && target < upto) {
-      rank = before;
-      for(int v = begin; v < end; ++v) {
-        sum += kept(v, rank);
-        if(sum > target) {
-          done(row, v, m, s.c, (double)total / (double)(1ull << scale));
-          break;
-        }
-      }
+      done(a, v, total);
     }
   }
 };

@@ -36,6 +36,9 @@
 #ifndef PRAGMA_UNROLL
   #define PRAGMA_UNROLL _Pragma("unroll")
 #endif
+#ifndef PRAGMA_NO_UNROLL
+  #define PRAGMA_NO_UNROLL _Pragma("clang loop unroll(disable)")
+#endif
 
 #define MGPU_ALIGN(bytes) __attribute__((aligned(bytes)))
 
