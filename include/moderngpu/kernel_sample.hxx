@@ -85,6 +85,15 @@ struct sample_row_t {
   int k;
   double p, least;
   bool by_count, by_mass;
+  // Quarter octaves, counted from where exp(z / T) is 1.  One product, rounded
+  // the same way wherever it is computed, so that a token is in one bin.
+  __forceinline__ MGPU_DEVICE float quarters(float z) const {
+    const float most = 268435456.f;
+    return __builtin_fmaxf(__builtin_fminf(z * (2 * c2), most), -most);
+  }
+  __forceinline__ MGPU_DEVICE static int bin(float quarters) {
+    return (int)__builtin_floorf(quarters);
+  }
   __forceinline__ MGPU_DEVICE bool all() const { return !by_count && !by_mass && !(least > 0); }
 };
 struct sample_settings_t {
@@ -104,7 +113,7 @@ struct sample_settings_t {
     s.least = __builtin_fminf(min_p ? min_p[r] : min_p_all, 1.f);
     if(!(t > 0)) { t = 1; s.k = 1; }
     s.c = 1.4426950408889634 / (double)t;
-    s.c2 = (float)__builtin_fmin(2 * s.c, 3e38);
+    s.c2 = (float)__builtin_fmin(2 * s.c, 1.5e38);
     s.by_count = s.k > 0 && s.k < vocab;
     s.by_mass = p < 1;
     s.p = __builtin_fmaxf(p, 0.f);
@@ -118,31 +127,76 @@ MGPU_DEVICE inline float sample_clean(float z) {
 }
 
 // A row is looked at in pieces of this many tokens first.
-enum { sample_piece_nt = 256, sample_piece = 8192, sample_bins = 64,
+enum { sample_piece_nt = 256, sample_piece = 8192,
+  sample_groups = 64,           // bins for the maxima of groups of tokens
+  sample_bins = 128,            // bins of a quarter octave
   sample_segments = 32,         // at most: waves x chunks of a piece
   sample_list = 2048,           // candidates of a piece that are kept
   sample_max_k = 1024 };        // largest k that candidates are found for
 
-// What a piece leaves for its row.
+// What the pieces leave for their row.
 struct sample_piece_t {
   double sum;                   // of 2^((z - max) c)
-  double segments[sample_segments];   // the same by 64 chunks of tokens
-  int table[sample_bins];       // tokens by half octaves of it below max
+  mass_t above;                 // mass that top-p keeps for sure
+  union {                       // by 64 chunks of tokens:
+    double segments[sample_segments]; // the sum
+    mass_t runs[sample_segments];     // what is left of `above` after min-p
+  };
+  float table[sample_bins];     // mass by quarter octaves, each in its own
   float max;
   int listed;                   // candidates; more than sample_list: too many
   unsigned short list[sample_list];   // where they are in the piece
 };
 
-// One CTA per piece reads its logits once and leaves their maximum and, by
-// what the row's settings need:
+template<typename type_t>
+struct sample_tokens_t {
+  enum { nt = sample_piece_nt, W = row_chunk_t<type_t>::width,
+    items = sample_piece / nt, chunks = items / W, waves = nt / 64 };
+  float z[items];
+
+  __forceinline__ MGPU_DEVICE sample_tokens_t(const type_t* row, int piece,
+    int vocab, int tid) {
+    row_chunk_t<type_t> ch[chunks];
+    PRAGMA_UNROLL
+    for(int c = 0; c < chunks; ++c) {
+      int v = piece * sample_piece + (c * nt + tid) * W;
+      ch[c].load(row + v, vocab - v, (type_t)-__builtin_inff());
+    }
+    PRAGMA_UNROLL
+    for(int i = 0; i < items; ++i)
+      z[i] = sample_clean((float)ch[i / W].x[i % W]);
+  }
+
+  // Lists the tokens with a bit set.  shared_count is 0, and all threads have
+  // seen that.
+  __forceinline__ MGPU_DEVICE static void list(unsigned in, int tid,
+    int& shared_count, sample_piece_t& to) {
+    int n = popc(in);
+    int at = wave_scan(n, plus_t<int>(), tid & 63);
+    int base = 0;
+    if(63 == (tid & 63) && at) base = atomicAdd(&shared_count, at);
+    at += readlane(base, 63) - n;
+    PRAGMA_UNROLL
+    for(int i = 0; i < items; ++i)
+      if(in >> i & 1) {
+        if(at < sample_list)
+          to.list[at] = (unsigned short)((i / W * nt + tid) * W + i % W);
+        ++at;
+      }
+    __syncthreads();
+    if(!tid) to.listed = shared_count;
+  }
+};
+
+// First launch: one CTA per piece reads its logits once and leaves their
+// maximum and, by what the row's settings need:
 //   top-k      the tokens that may be among the row's k largest.  The maxima of
 //              1024 groups of 8 tokens are counted in 64 bins between the
 //              largest and the smallest of them; the first bins that hold k
 //              maxima hold the piece's k largest tokens, and little else.
-//   top-p      the sum of its probabilities, and how many tokens there are in
-//              each half octave, which brackets how far down the kept ones
-//              reach.  (Sums by half octave would bracket it closer, but an
-//              LDS addition of floats takes 200 cycles a wave, a count 4.)
+//   top-p      the sum of its probabilities, and their sums by quarter octaves,
+//              as whole numbers (an LDS addition of floats takes 200 cycles a
+//              wave, one of integers 4).
 //   neither    the sum, and the sums of short runs of tokens.
 // The last two are bound by the 64-bit exponential, some 25 instructions a
 // token.
@@ -156,17 +210,16 @@ struct sample_piece_f {
 
   // The last bin for all that lies past it, and for NaN (infinity times 0).
   MGPU_DEVICE static int bin_of(float x) {
-    return (int)__builtin_fminf(x, sample_bins - 1);
+    return (int)__builtin_fminf(x, sample_groups - 1);
   }
 
   MGPU_DEVICE void operator()(int tid, int cta) const {
-    enum { nt = sample_piece_nt, W = row_chunk_t<type_t>::width,
-      items = sample_piece / nt, chunks = items / W, waves = nt / 64,
-      groups = items / 8 };
-    typedef row_chunk_t<type_t> chunk_t;
+    typedef sample_tokens_t<type_t> tokens_t;
+    enum { nt = sample_piece_nt, W = tokens_t::W, items = tokens_t::items,
+      chunks = tokens_t::chunks, waves = tokens_t::waves, groups = items / 8 };
     const float inf = __builtin_inff();
-    __shared__ int shared_table[sample_bins][64];
-    __shared__ int shared_hist[sample_bins];
+    __shared__ unsigned shared_table[sample_bins][64];
+    __shared__ int shared_hist[sample_groups];
     __shared__ float shared_max[waves], shared_min[waves];
     __shared__ double shared_sum[waves];
     __shared__ int shared_cut, shared_count;
@@ -174,19 +227,8 @@ struct sample_piece_f {
     int lane = tid & 63;
     sample_row_t s = settings.row(row, vocab);
     sample_piece_t& mine = out[cta];
-    const type_t* zs = logits + row * stride;
-
-    float z[items];
-    {
-      chunk_t ch[chunks];
-      PRAGMA_UNROLL
-      for(int c = 0; c < chunks; ++c) {
-        int v = piece * sample_piece + (c * nt + tid) * W;
-        ch[c].load(zs + v, vocab - v, (type_t)-inf);
-      }
-      PRAGMA_UNROLL
-      for(int i = 0; i < items; ++i) z[i] = sample_clean((float)ch[i / W].x[i % W]);
-    }
+    tokens_t tokens(logits + row * stride, piece, vocab, tid);
+    const float (&z)[items] = tokens.z;
     float group[groups];
     float m = -inf;
     PRAGMA_UNROLL
@@ -196,7 +238,7 @@ struct sample_piece_f {
       for(int i = 1; i < 8; ++i) group[g] = __builtin_fmaxf(group[g], z[8 * g + i]);
       m = __builtin_fmaxf(m, group[g]);
     }
-    if(tid < sample_bins) shared_hist[tid] = 0;
+    if(tid < sample_groups) shared_hist[tid] = 0;
     if(!tid) shared_count = 0;
     m = cta_allreduce<nt>(m, float_max_t(), tid, shared_max);
     if(!tid) mine.max = m;
@@ -215,7 +257,7 @@ struct sample_piece_f {
       for(int g = 0; g < groups; ++g)
         if(group[g] >= low) least = __builtin_fminf(least, group[g]);
       least = -cta_allreduce<nt>(-least, float_max_t(), tid, shared_min);
-      float per = least < m ? (sample_bins - 1) / (m - least) : 0.f;
+      float per = least < m ? (sample_groups - 1) / (m - least) : 0.f;
       PRAGMA_UNROLL
       for(int g = 0; g < groups; ++g)
         if(group[g] >= low)
@@ -224,54 +266,44 @@ struct sample_piece_f {
       if(tid < 64) {
         int upto = wave_scan(shared_hist[tid], plus_t<int>(), tid);
         lanemask_t enough = ballot(upto >= s.k);
-        if(!tid) shared_cut = enough ? ffs(enough) - 1 : sample_bins;
+        if(!tid) shared_cut = enough ? ffs(enough) - 1 : sample_groups;
       }
       __syncthreads();
-      float cut = shared_cut < sample_bins - 1 ? shared_cut + 1.f : inf;
-      int n = 0;
+      float cut = shared_cut < sample_groups - 1 ? shared_cut + 1.f : inf;
       unsigned in = 0;
       PRAGMA_UNROLL
       for(int i = 0; i < items; ++i)
-        if(z[i] >= low && z[i] > -inf && (cut == inf || (m - z[i]) * per < cut)) {
+        if(z[i] >= low && z[i] > -inf && (cut == inf || (m - z[i]) * per < cut))
           in |= 1u << i;
-          ++n;
-        }
-      int at = wave_scan(n, plus_t<int>(), lane);
-      int base = 0;
-      if(63 == lane) base = atomicAdd(&shared_count, at);
-      at += readlane(base, 63) - n;
-      PRAGMA_UNROLL
-      for(int i = 0; i < items; ++i)
-        if(in >> i & 1) {
-          if(at < sample_list)
-            mine.list[at] = (unsigned short)((i / W * nt + tid) * W + i % W);
-          ++at;
-        }
-      __syncthreads();
-      if(!tid) mine.listed = shared_count;
+      tokens_t::list(in, tid, shared_count, mine);
       return;
     }
 
-    bool all = s.all(), count = s.by_count || s.by_mass;
-    if(!all && !count) return;
-    if(count) {
+    bool all = s.all();
+    if(!all && (s.by_count || !s.by_mass)) return;
+    if(!all) {
       for(int i = tid; i < sample_bins * 64; i += nt)
         (&shared_table[0][0])[i] = 0;
       __syncthreads();
-      // Every lane has a column of the table: no two add at one address.
+      // Every lane has a column of the table: no two add at one address, and
+      // none gets past 128 * 2^24.
+      int top = sample_row_t::bin(s.quarters(m));
       PRAGMA_UNROLL
-      for(int i = 0; i < items; ++i)
-        if(z[i] > -inf)
-          atomicAdd(&shared_table[bin_of((m - z[i]) * s.c2)][lane], 1);
+      for(int i = 0; i < items; ++i) {
+        float q = s.quarters(z[i]);
+        int b = sample_row_t::bin(q), down = top - b;
+        if(z[i] > -inf && down < sample_bins)
+          atomicAdd(&shared_table[down][lane], (unsigned)
+            (16777216.f * __builtin_amdgcn_exp2f(.25f * (q - b) - .25f)));
+      }
       __syncthreads();
-      // Four threads a bin.
-      int bin = tid / 4, n = 0;
-      for(int i = 0; i < 16; ++i)
-        n += shared_table[bin][(tid & 3) * 16 + ((i + bin) & 15)];
-      n += dpp_move<dpp_quad_xor1>(n, n);
-      n += dpp_move<dpp_quad_xor2>(n, n);
-      if(!(tid & 3)) mine.table[bin] = n;
-      if(s.by_count) return;
+      // Two threads a bin.
+      int bin = tid / 2;
+      float x = 0;
+      for(int i = 0; i < 32; ++i)
+        x += shared_table[bin][(tid & 1) * 32 + ((i + bin) & 31)];
+      x += dpp_move<dpp_quad_xor1>(x, x);
+      if(!(tid & 1)) mine.table[bin] = x * (1 / 16777216.f);
     }
     sample_exp2_t exp2;
     double sum = 0;
@@ -298,11 +330,144 @@ struct sample_piece_f {
   }
 };
 
-// One CTA per row finishes it.  Where the tokens that may be kept are few, they
-// are listed in LDS and everything happens on the list.  Otherwise the row is
-// read again: a border found by top-k or top-p is first bracketed by the counts
-// per half octave, the tokens above the bracket are added up, those inside are
-// listed, and the border is found among them.
+// Probabilities as whole numbers.
+struct sample_scale_t {
+  int scale;
+  __forceinline__ MGPU_DEVICE double one() const {
+    return (double)(1ull << scale);
+  }
+  __forceinline__ MGPU_DEVICE mass_t whole(double share) const {
+    return (mass_t)(share * one() + .5);
+  }
+  // Octaves below the largest logit at which no probability is left.
+  __forceinline__ MGPU_DEVICE int nothing_left() const { return scale + 2; }
+};
+
+// Second launch, for rows with top-p or min-p but no top-k: with the sums of
+// all its pieces, a row's border lies in one quarter octave (two, should a sum
+// come within rounding of it).  One CTA per piece adds up the tokens above, by
+// runs, and lists those in the border's bins.  Without top-p, what is within
+// reach of min-p counts as above.
+template<typename type_t>
+struct sample_weigh_f {
+  const type_t* logits;
+  int64_t stride;
+  int vocab, pieces;
+  sample_scale_t scale;
+  sample_settings_t settings;
+  sample_piece_t* out;
+
+  MGPU_DEVICE void operator()(int tid, int cta) const {
+    typedef sample_tokens_t<type_t> tokens_t;
+    enum { nt = sample_piece_nt, W = tokens_t::W, items = tokens_t::items,
+      chunks = tokens_t::chunks, waves = tokens_t::waves };
+    const float inf = __builtin_inff();
+    __shared__ float shared_max[waves], shared_scan[waves];
+    __shared__ double shared_sum[waves];
+    __shared__ mass_t shared_above[waves];
+    __shared__ int shared_less[2][waves], shared_count;
+    int row = cta / pieces, piece = cta % pieces;
+    int lane = tid & 63, wave = tid / 64;
+    sample_row_t s = settings.row(row, vocab);
+    if(s.by_count || s.all()) return;
+    sample_piece_t& mine = out[cta];
+    const sample_piece_t* of_row = out + (int64_t)row * pieces;
+    tokens_t tokens(logits + row * stride, piece, vocab, tid);
+    const float (&z)[items] = tokens.z;
+
+    float m = -inf;
+    for(int p = tid; p < pieces; p += nt) m = __builtin_fmaxf(m, of_row[p].max);
+    if(!tid) shared_count = 0;
+    m = cta_allreduce<nt>(m, float_max_t(), tid, shared_max);
+    if(m == -inf) return;
+    sample_exp2_t exp2;
+
+    // Bins below the row's top one: less than `low` are above the border, none
+    // past `high` holds a kept token.
+    // Far from zero the bins' numbers are rounded: by 2^-24 of them, twice.
+    float q = s.quarters(m), far = __builtin_fabsf(q) + 4 * sample_bins;
+    int top = sample_row_t::bin(q), slack = 1 + (int)(3e-7f * far);
+    int low = 0x7fffffff, high = 4 * scale.nothing_left();
+    if(s.least > 0) high = min(high, (int)(-4 * (float)log2(s.least)));
+    high += slack;
+    if(s.by_mass) {
+      double sum = 0;
+      for(int p = tid; p < pieces; p += nt)
+        if(of_row[p].max > -inf)
+          sum += of_row[p].sum * exp2(((double)of_row[p].max - (double)m) * s.c);
+      sum = wave_allreduce(sum, plus_t<double>(), lane);
+      if(!lane) shared_sum[wave] = sum;
+      float x = 0;
+      for(int p = 0; p < pieces; ++p) {
+        int b = tid - (top - sample_row_t::bin(s.quarters(of_row[p].max)));
+        if(b >= 0 && b < sample_bins) x += of_row[p].table[b];
+      }
+      // The top of bin tid, relative to the largest logit.
+      x *= __builtin_amdgcn_exp2f(.25f * (top + 1 - tid - q));
+      float upto = wave_scan(x, plus_t<float>(), lane);
+      if(63 == lane) shared_scan[wave] = upto;
+      __syncthreads();
+      sum = shared_sum[0];
+      PRAGMA_UNROLL
+      for(int w = 1; w < waves; ++w) sum += shared_sum[w];
+      for(int w = 0; w < wave; ++w) upto += shared_scan[w];
+      float want = (float)(s.p * sum);
+      float margin = 1.0001f + 1e-6f * pieces + 4e-8f * far;
+      int less = popc(ballot(upto * margin < want));
+      int reached = popc(ballot(upto < want * margin));
+      if(!lane) {
+        shared_less[0][wave] = less;
+        shared_less[1][wave] = reached;
+      }
+      __syncthreads();
+      less = reached = 0;
+      PRAGMA_UNROLL
+      for(int w = 0; w < waves; ++w) {
+        less += shared_less[0][w];
+        reached += shared_less[1][w];
+      }
+      // A piece's table ends after sample_bins bins; further down the sums are
+      // not all there.
+      low = margin < 2 ? min(less, sample_bins - 1) : 0;
+      if(margin < 2 && reached < sample_bins) high = min(high, reached);
+    }
+
+    unsigned in = 0;
+    mass_t above = 0;
+    PRAGMA_UNROLL
+    for(int c = 0; c < chunks; ++c) {
+      mass_t run = 0;
+      PRAGMA_UNROLL
+      for(int i = c * W; i < c * W + W; ++i) {
+        int down = top - sample_row_t::bin(s.quarters(z[i]));
+        if(!(z[i] > -inf) || down > high) continue;
+        if(down < low) {
+          double e = exp2(((double)z[i] - (double)m) * s.c);
+          mass_t w = scale.whole(e);
+          above += w;
+          run += e >= s.least || z[i] == m ? w : 0;
+        } else
+          in |= 1u << i;
+      }
+      run = wave_allreduce(run, plus_t<mass_t>(), lane);
+      if(!lane) mine.runs[c * waves + wave] = run;
+    }
+    above = wave_allreduce(above, plus_t<mass_t>(), lane);
+    if(!lane) shared_above[wave] = above;
+    tokens_t::list(in, tid, shared_count, mine);
+    if(!tid) {
+      PRAGMA_UNROLL
+      for(int w = 1; w < waves; ++w) above += shared_above[w];
+      mine.above = above;
+    }
+  }
+};
+
+// Last launch: one CTA per row finishes it on the listed candidates, in LDS.
+// Where there are too many (k past sample_max_k, many equal logits, a
+// temperature at which all are nearly equal), it reads the row again: a border
+// is bracketed by the counts per half octave, the tokens above the bracket are
+// added up, those inside are listed, and the border is found among them.
 enum { sample_nt = 1024, sample_candidates = 16384, sample_row_bins = 128 };
 
 // Which tokens are kept: those with a larger key, and of those with this one
@@ -326,7 +491,7 @@ struct sample_row_f {
   const type_t* logits;
   int64_t stride;
   int vocab, pieces;
-  int scale;
+  sample_scale_t scale;
   const float* uniform;
   sample_settings_t settings;
   const sample_piece_t* from;
@@ -350,6 +515,7 @@ struct sample_row_f {
     int wave_int[num_waves];
     mass_t above, at;
     unsigned digit;
+    mass_t runs[nt];
     int listed, picked;
     int bracket[2];
     double rest;
@@ -369,7 +535,7 @@ struct sample_row_f {
     return sample_exp2_t()(((double)z - (double)a.m) * a.s.c);
   }
   __forceinline__ MGPU_DEVICE mass_t whole(double share) const {
-    return (mass_t)(share * (double)(1ull << scale) + .5);
+    return scale.whole(share);
   }
   // What a kept token has after min-p.
   __forceinline__ MGPU_DEVICE mass_t final_mass(const at_t& a, float z) const {
@@ -408,26 +574,28 @@ struct sample_row_f {
     return before + x;
   }
 
-  // get(i, value, weight) says whether entry i of [0, n) counts.  Returns the
-  // smallest value up to which, in ascending order, the weights sum up to
-  // `want` (which their total reaches), the sum in front of it and its own.
-  template<typename get_t>
-  __forceinline__ MGPU_DEVICE unsigned select(int n, int bits, mass_t want, get_t get, int tid,
-    shared_t& shared, mass_t& above, mass_t& at) const {
-    unsigned prefix = 0;
+  // value(i, x) says whether entry i of [0, n) counts, and its value; weight(i)
+  // is its weight.  Finds the smallest value up to which, in ascending order,
+  // the weights sum up to `want`, the sum in front of it and its own; false
+  // if they do not.
+  template<typename value_t, typename weight_t>
+  __forceinline__ MGPU_DEVICE bool select(int n, int bits, mass_t want,
+    value_t value, weight_t weight, int tid, shared_t& shared,
+    unsigned& found, mass_t& above, mass_t& at) const {
+    found = 0;
     above = 0;
     int left = bits;
     do {
       int width = min(left, 10), shift = left - width;
       __syncthreads();
       shared.hist[tid] = 0;
+      if(!tid) shared.digit = nt;
       __syncthreads();
       for(int i = tid; i < n; i += nt) {
-        unsigned value;
-        mass_t weight;
-        if(get(i, value, weight) &&
-          (unsigned long long)value >> left == (unsigned long long)prefix >> left)
-          atomicAdd(&shared.hist[(value >> shift) & ((1u << width) - 1)], weight);
+        unsigned x;
+        if(value(i, x) &&
+          (unsigned long long)x >> left == (unsigned long long)found >> left)
+          atomicAdd(&shared.hist[(x >> shift) & ((1u << width) - 1)], weight(i));
       }
       __syncthreads();
       mass_t mine = shared.hist[tid];
@@ -438,12 +606,13 @@ struct sample_row_f {
         shared.at = mine;
       }
       __syncthreads();
-      prefix |= shared.digit << shift;
+      if(nt == shared.digit) return false;
+      found |= shared.digit << shift;
       above = shared.above;
       at = shared.at;
       left = shift;
     } while(left > 0);
-    return prefix;
+    return true;
   }
 
   __forceinline__ MGPU_DEVICE void done(const at_t& a, int v, double total) const {
@@ -481,32 +650,19 @@ struct sample_row_f {
     float reach = nothing_left();
     if(a.s.least > 0)
       reach = __builtin_fminf(reach, .01f - 2 * (float)log2(a.s.least));
-    mass_t want = 0;
-    double sum = 0;
-    int n = sample_candidates + 1;
-    bool counted = true;              // the tables by half octave are there
-    if(a.s.by_count && a.s.k <= sample_max_k) {
-      n = gather_lists(a, shared);
-      counted = false;
-    } else {
-      if(a.s.by_count || a.s.by_mass) merge_tables(a, shared);
-      if(!a.s.by_count) {
-        float low, high = reach;
-        if(a.s.by_mass) {
-          sum = row_sum(a, shared);
-          want = goal(a.s.p * sum * (double)(1ull << scale));
-          bracket_mass(a, sum, low, high, shared);
-          high = __builtin_fminf(high, reach);
-        }
-        n = list_down_to(a, high, shared);
-      }
-    }
-    if(n <= sample_candidates) on_the_list(a, n, want, shared);
-    else on_the_row(a, reach, want, sum, counted, shared);
+    bool lists = !a.s.by_count || a.s.k <= sample_max_k;
+    int n = lists ? gather_lists(a, shared) : 0;
+    lists = lists && n <= sample_candidates;
+    double sum = !a.s.by_count && a.s.by_mass ? row_sum(a, shared) : 0;
+    if(!lists) on_the_row(a, reach, sum, shared);
+    else if(a.s.by_count) on_the_list(a, n, shared);
+    else on_weighed(a, n, sum, shared);
   }
 
   // Half octaves below the largest logit at which no probability is left.
-  __forceinline__ MGPU_DEVICE float nothing_left() const { return 2.f * (scale + 2); }
+  __forceinline__ MGPU_DEVICE float nothing_left() const {
+    return 2.f * scale.nothing_left();
+  }
 
   // Kept are those in front of whom there is less than x, a whole number
   // below its ceiling; the first always.
@@ -557,37 +713,13 @@ struct sample_row_f {
     }
   }
 
-  // The row's tokens by half octaves below its largest logit.
-  __forceinline__ MGPU_DEVICE void clear_tables(const at_t& a, shared_t& shared) const {
+  // The row's tokens by half octaves below its largest logit: bin b has those
+  // of b - 1 to b, the last one all the others.
+  __forceinline__ MGPU_DEVICE void count_row(const at_t& a, shared_t& shared)
+    const {
     __syncthreads();
-    if(a.tid < sample_row_bins) {
-      shared.most[a.tid] = 0;
-      shared.count[a.tid] = 0;
-    }
+    if(a.tid < sample_row_bins) shared.count[a.tid] = 0;
     __syncthreads();
-  }
-  // From the pieces' tables, shifted down to the row's largest logit: bin b
-  // has the tokens of b - 2 to b below it, the last one all the others.
-  __forceinline__ MGPU_DEVICE void merge_tables(const at_t& a, shared_t& shared) const {
-    clear_tables(a, shared);
-    for(int i = a.tid; i < pieces * sample_bins; i += nt) {
-      const sample_piece_t& from = a.piece[i / sample_bins];
-      int bin = i % sample_bins, n = 0;
-      float off = (a.m - from.max) * a.s.c2;
-      if(off < sample_row_bins) n = from.table[bin];
-      if(n) {
-        int to = sample_bins - 1 == bin ? sample_row_bins - 1 :
-          min((int)ceilf(off) + bin + 1, sample_row_bins - 1);
-        atomicAdd(&shared.most[to],
-          n * __builtin_amdgcn_exp2f(-.5f * (off + bin)));
-        atomicAdd(&shared.count[to], n);
-      }
-    }
-    __syncthreads();
-  }
-  // From the row.
-  __forceinline__ MGPU_DEVICE void count_row(const at_t& a, shared_t& shared) const {
-    clear_tables(a, shared);
     sweep(a, [&](int, const row_chunk_t<type_t> (&ch)[unroll]) {
       PRAGMA_UNROLL
       for(int i = 0; i < per_thread; ++i) {
@@ -605,15 +737,27 @@ struct sample_row_f {
   }
 
   // Brackets, in half octaves below the largest logit: every token less than
-  // `low` down is above the border, none more than `high` down is.
-  __forceinline__ MGPU_DEVICE void store_bracket(const at_t& a, int before, int last,
-    float& low, float& high, shared_t& shared) const {
-    // `before` bins are in front of the border, and hold every token down to
-    // before - 3 (a piece's tokens past its 63rd bin are in the last bin); the
-    // border is in bin `last` at most.
-    if(!a.tid) {
-      shared.bracket[0] = min(before - 3, sample_bins - 2);
-      shared.bracket[1] = last;
+  // `low` down is above the border, none more than `high` down is.  `before`
+  // bins are in front of the border, and hold every token down to before - 1;
+  // the border is in bin `last` at most.  Where the list has room for all, nothing is taken to
+  // be above.
+  __forceinline__ MGPU_DEVICE void bracket(const at_t& a, bool by_mass,
+    double sum, float& low, float& high, shared_t& shared) const {
+    if(a.tid < 64) {
+      int x = shared.count[2 * a.tid], y = shared.count[2 * a.tid + 1];
+      int upto = wave_scan(x + y, plus_t<int>(), a.tid);
+      int before, last;
+      if(by_mass)
+        bracket_mass(a, sum, before, last, shared);
+      else
+        before = last = popc(ballot(upto - y < a.s.k)) + popc(ballot(upto < a.s.k));
+      last = min(last, sample_row_bins - 1);
+      int listed = readlane(upto, last / 2) - (last & 1 ? 0 : readlane(y, last / 2));
+      if(!a.tid) {
+        shared.bracket[0] = listed <= sample_candidates ? -1 :
+          before - 1 - 1;          // (one for rounding)
+        shared.bracket[1] = last;
+      }
     }
     __syncthreads();
     low = shared.bracket[0];
@@ -621,39 +765,18 @@ struct sample_row_f {
       shared.bracket[1] + .01f;
     __syncthreads();
   }
-  __forceinline__ MGPU_DEVICE void bracket(const at_t& a, bool by_mass,
-    double sum, float& low, float& high, shared_t& shared) const {
-    if(by_mass) bracket_mass(a, sum, low, high, shared);
-    else bracket_count(a, low, high, shared);
-  }
-  __forceinline__ MGPU_DEVICE void bracket_count(const at_t& a, float& low, float& high,
-    shared_t& shared) const {
-    int less = 0;
-    if(a.tid < 64) {
-      int x = shared.count[2 * a.tid], y = shared.count[2 * a.tid + 1];
-      int upto = wave_scan(x + y, plus_t<int>(), a.tid);
-      less = popc(ballot(upto - y < a.s.k)) + popc(ballot(upto < a.s.k));
-    }
-    store_bracket(a, less, less, low, high, shared);
-  }
-  // Sums of 32-bit floats of up to 64 * pieces terms are off by 4e-6 * pieces
-  // at most.
-  __forceinline__ MGPU_DEVICE void bracket_mass(const at_t& a, double sum, float& low,
-    float& high, shared_t& shared) const {
-    int before = 0, last = 0;
-    if(a.tid < 64) {
-      float margin = 1.0001f + 1e-5f * pieces;
-      float x = shared.most[2 * a.tid], y = shared.most[2 * a.tid + 1];
-      float upto = wave_scan(x + y, plus_t<float>(), a.tid);
-      float want = (float)(a.s.p * sum) / margin;
-      before = popc(ballot(upto - y < want)) + popc(ballot(upto < want));
-      // Bins with more than 1 - p from them on.
-      x = shared.most[127 - 2 * a.tid], y = shared.most[126 - 2 * a.tid];
-      upto = wave_scan(x + y, plus_t<float>(), a.tid);
-      float rest = (float)((1 - a.s.p) * sum) / margin;
-      last = popc(ballot(upto - y > rest)) + popc(ballot(upto > rest)) - 1;
-    }
-    store_bracket(a, before, last, low, high, shared);
+  __forceinline__ MGPU_DEVICE void bracket_mass(const at_t& a, double sum,
+    int& before, int& last, shared_t& shared) const {
+    const float margin = 1.0001f;         // 128 terms
+    float x = shared.most[2 * a.tid], y = shared.most[2 * a.tid + 1];
+    float upto = wave_scan(x + y, plus_t<float>(), a.tid);
+    float want = (float)(a.s.p * sum) / margin;
+    before = popc(ballot(upto - y < want)) + popc(ballot(upto < want));
+    // Bins with more than 1 - p from them on.
+    x = shared.most[127 - 2 * a.tid], y = shared.most[126 - 2 * a.tid];
+    upto = wave_scan(x + y, plus_t<float>(), a.tid);
+    float rest = (float)((1 - a.s.p) * sum) / margin;
+    last = popc(ballot(upto - y > rest)) + popc(ballot(upto > rest)) - 1;
   }
 
   // The row's sum of 2^((z - m) c).
@@ -686,49 +809,67 @@ struct sample_row_f {
       }
   }
 
-  // Lists the tokens down to `high` half octaves below the largest logit and
-  // returns how many there are; more than sample_candidates: not all listed.
-  __forceinline__ MGPU_DEVICE int list_down_to(const at_t& a, float high,
-    shared_t& shared) const {
-    __syncthreads();
-    if(!a.tid) shared.listed = 0;
-    __syncthreads();
-    sweep(a, [&](int v, const row_chunk_t<type_t> (&ch)[unroll]) {
-      unsigned in = 0;
-      PRAGMA_UNROLL
-      for(int i = 0; i < per_thread; ++i) {
-        float x = sample_clean((float)ch[i / W].x[i % W]);
-        // (NaN, for a difference past the largest float at c2 = 0, is in)
-        if(x > -__builtin_inff() && !((a.m - x) * a.s.c2 > high)) in |= 1u << i;
-      }
-      append(a, v, ch, in, shared);
-    });
-    __syncthreads();
-    return shared.listed;
+  // The run that token v is in: 64 * W tokens, or a power of two of those.
+  __forceinline__ MGPU_DEVICE int run_bits() const {
+    int bits = 31 - clz(64u * W);
+    while((vocab - 1) >> bits >= nt) ++bits;
+    return bits;
   }
 
-  // The same within the cut, without the tokens less than `low` down: those are
-  // added up (counted, or their mass).
+  // Of the tokens within the cut, down to `high` half octaves below the largest
+  // logit: those less than `low` down are added up (counted, or their mass),
+  // and what they have after min-p goes to their runs; the others are listed.
+  // listed > sample_candidates: there were that many, not all listed.
   __forceinline__ MGPU_DEVICE mass_t add_above(const at_t& a, bool by_mass,
     sample_cut_t cut, float low, float high, int& listed, shared_t& shared)
     const {
+    int bits = run_bits();
     __syncthreads();
     if(!a.tid) shared.listed = 0;
+    shared.runs[a.tid] = 0;
     __syncthreads();
     mass_t sum = 0;
     sweep(a, [&](int v, const row_chunk_t<type_t> (&ch)[unroll]) {
       unsigned in = 0;
       PRAGMA_UNROLL
-      for(int i = 0; i < per_thread; ++i) {
-        float x = sample_clean((float)ch[i / W].x[i % W]);
-        float down = (a.m - x) * a.s.c2;
-        if(x > -__builtin_inff() && !(down > high) &&
-          cut.keeps(sample_key(x), v + i / W * nt * W + i % W)) {
-          if(!(down < low)) in |= 1u << i;
-          else sum += by_mass ? whole(share(a, x)) : 1;
+      for(int c = 0; c < unroll; ++c) {
+        mass_t run = 0;
+        PRAGMA_UNROLL
+        for(int i = 0; i < W; ++i) {
+          float x = sample_clean((float)ch[c].x[i]);
+          // (NaN, for a difference past the largest float at c2 = 0, is in)
+          float down = (a.m - x) * a.s.c2;
+          if(x > -__builtin_inff() && !(down > high) &&
+            cut.keeps(sample_key(x), v + c * nt * W + i)) {
+            if(!(down < low)) in |= 1u << (c * W + i);
+            else {
+              double e = share(a, x);
+              mass_t w = whole(e);
+              sum += by_mass ? w : 1;
+              run += e >= a.s.least || x == a.m ? w : 0;
+            }
+          }
+        }
+        if(low > 0) {
+          run = wave_allreduce(run, plus_t<mass_t>(), a.tid & 63);
+          if(!(a.tid & 63) && run)
+            atomicAdd(&shared.runs[(v + c * nt * W) >> bits], run);
         }
       }
-      append(a, v, ch, in, shared);
+      int n = popc(in);
+      int at = wave_scan(n, plus_t<int>(), a.tid & 63);
+      int base = 0;
+      if(63 == (a.tid & 63) && at) base = atomicAdd(&shared.listed, at);
+      at += readlane(base, 63) - n;
+      PRAGMA_UNROLL
+      for(int i = 0; i < per_thread; ++i)
+        if(in >> i & 1) {
+          if(at < sample_candidates) {
+            shared.key[at] = sample_key((float)ch[i / W].x[i % W]);
+            shared.index[at] = v + i / W * nt * W + i % W;
+          }
+          ++at;
+        }
     });
     sum = fold(sum, plus_t<mass_t>(), a.tid, shared.wave_mass);
     listed = shared.listed;
@@ -736,10 +877,9 @@ struct sample_row_f {
   }
 
   // The border among n listed tokens, of which those within `cut` count: kept
-  // are the ones in front of whom there is less than `want`, which they reach
-  // together.
-  __forceinline__ MGPU_DEVICE sample_cut_t border_of(const at_t& a, int n, bool by_mass,
-    sample_cut_t cut, mass_t want, shared_t& shared) const {
+  // are the ones in front of whom there is less than `want`.
+  __forceinline__ MGPU_DEVICE sample_cut_t border_of(const at_t& a, int n,
+    bool by_mass, sample_cut_t cut, mass_t want, shared_t& shared) const {
     unsigned best = rank_of(sample_key(a.m));
     auto down = [&](int i) { return best - rank_of(shared.key[i]); };
     unsigned deepest = 0;
@@ -747,115 +887,146 @@ struct sample_row_f {
     deepest = fold(deepest, maximum_t<unsigned>(), a.tid,
       (unsigned (&)[num_waves])shared.wave_int);
     mass_t above, at;
-    unsigned to = select(n, 32 - clz(deepest), want,
-      [&](int i, unsigned& value, mass_t& weight) {
-        if(!cut.keeps(shared.key[i], shared.index[i])) return false;
-        value = down(i);
-        weight = by_mass ? whole(share(a, sample_value(shared.key[i]))) : 1;
-        return true;
-      }, a.tid, shared, above, at);
+    unsigned to;
+    if(!select(n, 32 - clz(deepest), want,
+      [&](int i, unsigned& x) {
+        x = down(i);
+        return cut.keeps(shared.key[i], shared.index[i]);
+      },
+      [&](int i) {
+        return by_mass ? whole(share(a, sample_value(shared.key[i]))) : 1;
+      }, a.tid, shared, to, above, at)) return cut;
     sample_cut_t found = { key_of(best - to), vocab };
     mass_t each = by_mass ? whole(share(a, sample_value(found.key))) : 1;
     mass_t ties = (want - above + each - 1) / each;
     if(found.key == cut.key) found.last = cut.last;
     if(ties * each < at) {
       sample_cut_t ends = found;
-      found.last = (int)select(n, 32 - clz((unsigned)vocab - 1), ties,
-        [&](int i, unsigned& value, mass_t& weight) {
-          value = shared.index[i];
-          weight = 1;
-          return shared.key[i] == ends.key && (int)value <= ends.last;
-        }, a.tid, shared, above, at);
+      select(n, 32 - clz((unsigned)vocab - 1), ties,
+        [&](int i, unsigned& x) {
+          x = shared.index[i];
+          return shared.key[i] == ends.key && (int)x <= ends.last;
+        },
+        [&](int) { return (mass_t)1; }, a.tid, shared, to, above, at);
+      found.last = (int)to;
     }
     return found;
   }
 
-  __forceinline__ MGPU_DEVICE mass_t mass_within(const at_t& a, int n,
-    sample_cut_t cut, shared_t& shared) const {
-    mass_t all = 0;
-    for(int i = a.tid; i < n; i += nt)
-      if(cut.keeps(shared.key[i], shared.index[i]))
-        all += whole(share(a, sample_value(shared.key[i])));
-    return fold(all, plus_t<mass_t>(), a.tid, shared.wave_mass);
-  }
-
-  // n candidates that hold every token to be kept.  want: top-p's without
-  // top-k.
-  __forceinline__ MGPU_DEVICE void on_the_list(const at_t& a, int n, mass_t want,
+  // n candidates that hold every token to be kept.
+  __forceinline__ MGPU_DEVICE void on_the_list(const at_t& a, int n,
     shared_t& shared) const {
     __syncthreads();
     sample_cut_t cut = { 0, vocab };
     PRAGMA_NO_UNROLL
     for(int by_mass = 0; by_mass < 2; ++by_mass) {
-      if(by_mass ? !a.s.by_mass : !a.s.by_count) continue;
-      mass_t all = n;
+      mass_t want = a.s.k;
       if(by_mass) {
-        all = mass_within(a, n, cut, shared);
-        if(a.s.by_count) want = goal(a.s.p * (double)all);
+        if(!a.s.by_mass) break;
+        mass_t all = 0;
+        for(int i = a.tid; i < n; i += nt)
+          if(cut.keeps(shared.key[i], shared.index[i]))
+            all += whole(share(a, sample_value(shared.key[i])));
+        all = fold(all, plus_t<mass_t>(), a.tid, shared.wave_mass);
+        want = goal(a.s.p * (double)all);
       }
-      mass_t need = by_mass ? want : (mass_t)a.s.k;
-      if(need < all) cut = border_of(a, n, by_mass, cut, need, shared);
+      cut = border_of(a, n, by_mass, cut, want, shared);
     }
-    auto mass = [&](int i) -> mass_t {
-      return cut.keeps(shared.key[i], shared.index[i]) ?
-        final_mass(a, sample_value(shared.key[i])) : 0;
-    };
-    mass_t total = 0;
-    for(int i = a.tid; i < n; i += nt) total += mass(i);
-    total = fold(total, plus_t<mass_t>(), a.tid, shared.wave_mass);
-    mass_t target = min((mass_t)(a.u * (double)total), total - 1), above, at;
-    int v = (int)select(n, 32 - clz((unsigned)vocab - 1), target + 1,
-      [&](int i, unsigned& value, mass_t& weight) {
-        value = shared.index[i];
-        weight = mass(i);
-        return weight > 0;
-      }, a.tid, shared, above, at);
-    if(!a.tid) done(a, v, (double)total / (double)(1ull << scale));
+    draw_from_list(a, n, cut, shared);
   }
 
-  // Too many for the list: one reading of the row per border (and one for the
-  // total between top-k and top-p), and one for the draw.  want, sum: top-p's
-  // without top-k.
-  __forceinline__ MGPU_DEVICE void on_the_row(const at_t& a, float reach,
-    mass_t want, double sum, bool counted, shared_t& shared) const {
-    enum { border_by_count, total, border_by_mass };
+  // What the second launch left: sums above the border, and a list around it.
+  __forceinline__ MGPU_DEVICE void on_weighed(const at_t& a, int n, double sum,
+    shared_t& shared) const {
+    enum { segments = sample_segments / (W / 4) };
+    int shift = run_bits() - (31 - clz(64u * W));
+    __syncthreads();
+    shared.runs[a.tid] = 0;
+    __syncthreads();
+    mass_t above = 0;
+    for(int i = a.tid; i < pieces * segments; i += nt) {
+      const sample_piece_t& from = a.piece[i / segments];
+      mass_t x = from.runs[i % segments];
+      if(x) atomicAdd(&shared.runs[i >> shift], x);
+      if(!(i % segments)) above += from.above;
+    }
     sample_cut_t cut = { 0, vocab };
+    if(a.s.by_mass) {
+      above = fold(above, plus_t<mass_t>(), a.tid, shared.wave_mass);
+      cut = border_of(a, n, true, cut, goal(a.s.p * sum * scale.one()) - above,
+        shared);
+    }
+    __syncthreads();
+    draw_from_runs(a, n, cut, shared);
+  }
+
+  // The draw from the listed tokens within the cut.
+  __forceinline__ MGPU_DEVICE void draw_from_list(const at_t& a, int n,
+    sample_cut_t cut, shared_t& shared) const {
+    auto mass = [&](int i) { return final_mass(a, sample_value(shared.key[i])); };
+    auto kept = [&](int i) { return cut.keeps(shared.key[i], shared.index[i]); };
+    mass_t total = 0;
+    for(int i = a.tid; i < n; i += nt) if(kept(i)) total += mass(i);
+    total = fold(total, plus_t<mass_t>(), a.tid, shared.wave_mass);
+    mass_t target = min((mass_t)(a.u * (double)total), total - 1), above, at;
+    unsigned v;
+    select(n, 32 - clz((unsigned)vocab - 1), target + 1,
+      [&](int i, unsigned& x) {
+        x = shared.index[i];
+        return kept(i);
+      }, mass, a.tid, shared, v, above, at);
+    if(!a.tid) done(a, (int)v, (double)total / scale.one());
+  }
+
+  // One reading of the row per border (and one for the total between top-k and
+  // top-p); the last one leaves what the draw needs.  sum: top-p's without
+  // top-k.
+  __forceinline__ MGPU_DEVICE void on_the_row(const at_t& a, float reach,
+    double sum, shared_t& shared) const {
+    enum { border_by_count, total, border_by_mass, min_p_alone };
+    sample_cut_t cut = { 0, vocab };
+    float low = -1;
+    int n = 0;
+    bool again = false;
     PRAGMA_NO_UNROLL
-    for(int step = border_by_count; step <= border_by_mass; ++step) {
+    for(int step = border_by_count; step <= min_p_alone; ++step) {
       bool by_mass = step != border_by_count;
-      if((step <= total && !a.s.by_count) || (by_mass && !a.s.by_mass))
-        continue;
-      float low = __builtin_inff(), high = nothing_left();
-      if(step != total) {
-        if(!counted) {
-          count_row(a, shared);
-          counted = true;
-        }
+      if(min_p_alone == step ? a.s.by_count || a.s.by_mass :
+        (step <= total && !a.s.by_count) || (by_mass && !a.s.by_mass)) continue;
+      float high = nothing_left();
+      if(total == step) low = __builtin_inff();
+      else if(min_p_alone == step) high = reach;
+      else {
+        count_row(a, shared);
         float down;
         bracket(a, by_mass, sum, low, down, shared);
-        high = __builtin_fminf(high, down);
+        // What lies past min-p's reach does not matter to the last border.
+        high = __builtin_fminf(down, by_mass || !a.s.by_mass ? reach : high);
       }
-      int n;
       mass_t above = add_above(a, by_mass, cut, low, high, n, shared);
-      if(step == total) {
-        want = goal(a.s.p * (double)above);
-        sum = (double)above / (double)(1ull << scale);
+      if(min_p_alone == step) {
+        if(n > sample_candidates) {
+          low = __builtin_inff();
+          add_above(a, by_mass, cut, low, high, n, shared);
+        }
+        break;
+      }
+      if(total == step) {
+        sum = (double)above / scale.one();
         continue;
       }
-      mass_t need = by_mass ? want : (mass_t)a.s.k;
-      if(n > sample_candidates) {
-        cut = border_on_row(a, by_mass, cut, need, shared);
-        counted = false;                      // hist lies over the tables
-      } else {
-        mass_t all = above + (by_mass ? mass_within(a, n, cut, shared) :
-          (mass_t)n);
-        if(need < all) {
-          cut = border_of(a, n, by_mass, cut, need - above, shared);
-          counted = false;
-        }
-      }
+      mass_t want = by_mass ? goal(a.s.p * sum * scale.one()) :
+        (mass_t)a.s.k;
+      again = n > sample_candidates;
+      cut = again ? border_on_row(a, by_mass, cut, want, shared) :
+        border_of(a, n, by_mass, cut, want - above, shared);
     }
-    draw_on_row(a, cut, reach, shared);
+    if(again) {
+      low = __builtin_inff();
+      add_above(a, false, cut, low, reach, n, shared);
+    }
+    if(low > 0) draw_from_runs(a, n, cut, shared);
+    else draw_from_list(a, n, cut, shared);
   }
 
   // The border by 8 bits of the key at a time: more tokens than fit the list
@@ -936,36 +1107,17 @@ struct sample_row_f {
     return found;
   }
 
-  // The draw from the row's tokens within the cut: their mass by runs of
-  // 64 * W tokens (or a power of two of those), the run that holds the target,
-  // the token.
-  __forceinline__ MGPU_DEVICE void draw_on_row(const at_t& a, sample_cut_t cut, float reach,
-    shared_t& shared) const {
-    enum { run = 64 * W };
-    int tid = a.tid, more = 0;
-    while((vocab - 1) / run >> more >= nt) ++more;
-    auto mass = [&](float x, int v) -> mass_t {
-      return x > -__builtin_inff() && !((a.m - x) * a.s.c2 > reach) &&
-        (!cut.key || cut.keeps(sample_key(x), v)) ? final_mass(a, x) : 0;
-    };
+  // The draw from the tokens that add_above put into the runs and the listed
+  // ones within the cut: the run that holds the target, the token in it.
+  __forceinline__ MGPU_DEVICE void draw_from_runs(const at_t& a, int n,
+    sample_cut_t cut, shared_t& shared) const {
+    int tid = a.tid, bits = run_bits();
+    for(int i = tid; i < n; i += nt)
+      if(cut.keeps(shared.key[i], shared.index[i]))
+        atomicAdd(&shared.runs[shared.index[i] >> bits],
+          final_mass(a, sample_value(shared.key[i])));
     __syncthreads();
-    shared.hist[tid] = 0;
-    __syncthreads();
-    sweep(a, [&](int v, const row_chunk_t<type_t> (&ch)[unroll]) {
-      PRAGMA_UNROLL
-      for(int c = 0; c < unroll; ++c) {
-        mass_t sum = 0;
-        int v0 = v + c * nt * W;
-        PRAGMA_UNROLL
-        for(int i = 0; i < W; ++i)
-          sum += mass(sample_clean((float)ch[c].x[i]), v0 + i);
-        sum = wave_allreduce(sum, plus_t<mass_t>(), tid & 63);
-        if(!(tid & 63) && sum)
-          atomicAdd(&shared.hist[v0 / run >> more], sum);
-      }
-    });
-    __syncthreads();
-    mass_t mine = shared.hist[tid];
+    mass_t mine = shared.runs[tid];
     mass_t upto = scan(mine, tid, shared.wave_mass);
     mass_t total = fold(mine, plus_t<mass_t>(), tid, shared.wave_mass);
     mass_t target = min((mass_t)(a.u * (double)total), total - 1);
@@ -976,15 +1128,17 @@ struct sample_row_f {
     __syncthreads();
     if(tid >= 64) return;
     mass_t rest = target - shared.above;
-    int first = (shared.picked << more) * run, end = vocab;
-    for(int v0 = first; v0 < end; v0 += run) {
+    for(int v0 = shared.picked << bits; v0 < vocab; v0 += 64 * W) {
       int v = v0 + tid * W;
       row_chunk_t<type_t> ch;
       ch.load(a.z + v, vocab - v, (type_t)-__builtin_inff());
       mass_t x[W], sum = 0;
       PRAGMA_UNROLL
-      for(int i = 0; i < W; ++i)
-        sum += x[i] = mass(sample_clean((float)ch.x[i]), v + i);
+      for(int i = 0; i < W; ++i) {
+        float z = sample_clean((float)ch.x[i]);
+        sum += x[i] = cut.keeps(sample_key(z), v + i) && z > -__builtin_inff() ?
+          final_mass(a, z) : 0;
+      }
       mass_t to = wave_scan(sum, plus_t<mass_t>(), tid);
       mass_t all = readlane(to, 63);
       if(rest < all) {
@@ -992,7 +1146,7 @@ struct sample_row_f {
         PRAGMA_UNROLL
         for(int i = 0; i < W; ++i) {
           if(to <= rest && rest < to + x[i])
-            done(a, v + i, (double)total / (double)(1ull << scale));
+            done(a, v + i, (double)total / scale.one());
           to += x[i];
         }
         return;
@@ -1102,8 +1256,12 @@ void sample_launch(const type_t* logits, int64_t stride, int rows, int vocab,
   sample_piece_t* from = (sample_piece_t*)workspace;
   sample_piece_f<type_t> look { logits, stride, vocab, pieces, settings, from };
   cta_launch<sample_piece_nt>(look, rows * pieces, context);
-  sample_row_f<type_t> draw { logits, stride, vocab, pieces, min(62 - bits, 50),
-    uniform, settings, from, token, logprob };
+  sample_scale_t scale { min(62 - bits, 50) };
+  sample_weigh_f<type_t> weigh { logits, stride, vocab, pieces, scale, settings,
+    from };
+  cta_launch<sample_piece_nt>(weigh, rows * pieces, context);
+  sample_row_f<type_t> draw { logits, stride, vocab, pieces, scale, uniform,
+    settings, from, token, logprob };
   cta_launch<sample_nt>(draw, rows, context);
 }
 
