@@ -172,11 +172,12 @@ MGPU_DEVICE inline void needed_here(const type_t& x) {
   asm volatile("" :: "v"(s.w[0]));
 }
 
-// Makes a constant a value in a vector register: what is added to a product
-// of 64-bit floats is otherwise moved there word by word before each use.
-MGPU_DEVICE inline double held_in_register(double x) {
-  asm("" : "+v"(x));
-  return x;
+// x * y + c with c from scalar registers.  (Left to itself the compiler takes
+// the two-address form and copies a constant c to vector registers each time.)
+MGPU_DEVICE inline double fma_constant(double x, double y, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(x), "v"(y), "s"(c));
+  return d;
 }
 
 template<typename type_t>

@@ -54,29 +54,35 @@ MGPU_HOST_DEVICE float sample_value(unsigned key) {
 // the polynomial that interpolates (2^f - 1) / f at 9 Chebyshev nodes.  NaN
 // (0 times infinity) gives 0.
 struct sample_exp2_t {
-  double a[8];
-
-  __forceinline__ MGPU_DEVICE sample_exp2_t() {
-    const double c[8] = { 1.3255224878668817e-06, 1.525268684626772e-05,
-      0.00015403455852453838, 0.0013333558179043112, 0.0096181291594025584,
-      0.055504108664760424, 0.24022650695812989, 0.69314718055994529 };
-    PRAGMA_UNROLL
-    for(int i = 0; i < 8; ++i) a[i] = held_in_register(c[i]);
-  }
   __forceinline__ MGPU_DEVICE double operator()(double y) const {
     const double magic = 6755399441055744.;           // 1.5 * 2^52
     y = __builtin_fmax(y, -1100.);
     double t = y + magic;
     double f = y - (t - magic);
-    double x = 1.0203121063391729e-07;
-    PRAGMA_UNROLL
-    for(int i = 0; i < 8; ++i) x = __builtin_fma(x, f, a[i]);
+    double x = fma_constant(f, 1.0203121063391729e-07, 1.3255224878668817e-06);
+    x = fma_constant(x, f, 1.525268684626772e-05);
+    x = fma_constant(x, f, 0.00015403455852453838);
+    x = fma_constant(x, f, 0.0013333558179043112);
+    x = fma_constant(x, f, 0.0096181291594025584);
+    x = fma_constant(x, f, 0.055504108664760424);
+    x = fma_constant(x, f, 0.24022650695812989);
+    x = fma_constant(x, f, 0.69314718055994529);
     x = __builtin_fma(x, f, 1.);
     long long bits;
     __builtin_memcpy(&bits, &t, 8);
     return __builtin_amdgcn_ldexp(x, (int)bits);
   }
 };
+
+// A row is looked at in pieces of this many tokens first.
+enum { sample_piece_nt = 256, sample_piece = 8192,
+  sample_groups = 64,           // bins for the maxima of groups of tokens
+  sample_bins = 128,            // bins of a quarter octave
+  sample_segments = 32,         // at most: waves x chunks of a piece
+  sample_list = 2048,           // candidates of a piece that are kept
+  sample_max_k = 1536,          // largest k that candidates are found for
+  sample_few = 256,             // largest that groups' maxima find them for
+  sample_candidates = 16384 };  // candidates of a row that fit its list
 
 // One row's settings.
 struct sample_row_t {
@@ -89,10 +95,14 @@ struct sample_row_t {
   // the same way wherever it is computed, so that a token is in one bin.
   __forceinline__ MGPU_DEVICE float quarters(float z) const {
     const float most = 268435456.f;
-    return __builtin_fmaxf(__builtin_fminf(z * (2 * c2), most), -most);
+    return __builtin_amdgcn_fmed3f(z * (2 * c2), -most, most);
   }
   __forceinline__ MGPU_DEVICE static int bin(float quarters) {
     return (int)__builtin_floorf(quarters);
+  }
+  // top-k: whether the row has to drop candidates of some pieces for others'.
+  __forceinline__ MGPU_DEVICE bool counted(int pieces) const {
+    return k > sample_few || k * pieces > sample_candidates / 2;
   }
   __forceinline__ MGPU_DEVICE bool all() const { return !by_count && !by_mass && !(least > 0); }
 };
@@ -126,13 +136,8 @@ MGPU_DEVICE inline float sample_clean(float z) {
   return z == z ? __builtin_fminf(z, 3.402823466e38f) : -__builtin_inff();
 }
 
-// A row is looked at in pieces of this many tokens first.
-enum { sample_piece_nt = 256, sample_piece = 8192,
-  sample_groups = 64,           // bins for the maxima of groups of tokens
-  sample_bins = 128,            // bins of a quarter octave
-  sample_segments = 32,         // at most: waves x chunks of a piece
-  sample_list = 2048,           // candidates of a piece that are kept
-  sample_max_k = 1024 };        // largest k that candidates are found for
+// Bins of keys, 32 of them for a factor of two in the logit.
+MGPU_HOST_DEVICE int sample_key_bin(unsigned key) { return (int)(key >> 18); }
 
 // What the pieces leave for their row.
 struct sample_piece_t {
@@ -142,7 +147,7 @@ struct sample_piece_t {
     double segments[sample_segments]; // the sum
     mass_t runs[sample_segments];     // what is left of `above` after min-p
   };
-  float table[sample_bins];     // mass by quarter octaves, each in its own
+  float table[sample_bins];     // by bins: sum, or number of tokens
   float max;
   int listed;                   // candidates; more than sample_list: too many
   unsigned short list[sample_list];   // where they are in the piece
@@ -190,10 +195,13 @@ struct sample_tokens_t {
 
 // First launch: one CTA per piece reads its logits once and leaves their
 // maximum and, by what the row's settings need:
-//   top-k      the tokens that may be among the row's k largest.  The maxima of
-//              1024 groups of 8 tokens are counted in 64 bins between the
-//              largest and the smallest of them; the first bins that hold k
-//              maxima hold the piece's k largest tokens, and little else.
+//   top-k      the tokens that may be among the row's k largest.  For few, the
+//              maxima of 1024 groups of 8 tokens are counted in 64 bins between
+//              the largest and the smallest of them; the first bins that hold k
+//              maxima hold the piece's k largest tokens, and little else.  For
+//              more, and for the row to drop what the other pieces outdo, the
+//              tokens are counted by the upper bits of their keys, 32 bins for
+//              a factor of two.
 //   top-p      the sum of its probabilities, and their sums by quarter octaves,
 //              as whole numbers (an LDS addition of floats takes 200 cycles a
 //              wave, one of integers 4).
@@ -249,7 +257,49 @@ struct sample_piece_f {
       return;
     }
 
-    if(s.by_count && s.k <= sample_max_k) {
+    int bin = tid / 2;                // two threads a bin
+    if(s.by_count ? s.k <= sample_max_k && s.counted(pieces) : s.by_mass) {
+      for(int i = tid; i < sample_bins * 64; i += nt)
+        (&shared_table[0][0])[i] = 0;
+      __syncthreads();
+    }
+    auto add_columns = [&]() {
+      float x = 0;
+      for(int i = 0; i < 32; ++i)
+        x += shared_table[bin][(tid & 1) * 32 + ((i + bin) & 31)];
+      return x + dpp_move<dpp_quad_xor1>(x, x);
+    };
+
+    if(s.by_count) {
+      if(s.k > sample_max_k) return;
+      if(s.counted(pieces)) {
+        // Every lane has a column of the table: no two add at one address.
+        int top = sample_key_bin(sample_key(m));
+        PRAGMA_UNROLL
+        for(int i = 0; i < items; ++i) {
+          int down = top - sample_key_bin(sample_key(z[i]));
+          if(z[i] > -inf && down < sample_bins)
+            atomicAdd(&shared_table[down][lane], 1u);
+        }
+        __syncthreads();
+        float x = add_columns();
+        if(!(tid & 1)) mine.table[bin] = x;
+        if(s.k > sample_few) {
+          // The bin that holds the k-th.
+          float upto = wave_scan(tid & 1 ? 0.f : x, plus_t<float>(), lane);
+          if(63 == lane) shared_max[tid / 64] = upto;
+          __syncthreads();
+          for(int w = 0; w < tid / 64; ++w) upto += shared_max[w];
+          int less = __syncthreads_count(!(tid & 1) && upto < s.k);
+          unsigned in = 0;
+          PRAGMA_UNROLL
+          for(int i = 0; i < items; ++i)
+            if(z[i] > -inf && (less == sample_bins ||
+              top - sample_key_bin(sample_key(z[i])) <= less)) in |= 1u << i;
+          tokens_t::list(in, tid, shared_count, mine);
+          return;
+        }
+      }
       // Nothing further below than this has a probability left: 52 octaves.
       float low = m - 104.f / s.c2;
       float least = m;
@@ -281,38 +331,25 @@ struct sample_piece_f {
 
     bool all = s.all();
     if(!all && (s.by_count || !s.by_mass)) return;
-    if(!all) {
-      for(int i = tid; i < sample_bins * 64; i += nt)
-        (&shared_table[0][0])[i] = 0;
-      __syncthreads();
-      // Every lane has a column of the table: no two add at one address, and
-      // none gets past 128 * 2^24.
-      int top = sample_row_t::bin(s.quarters(m));
-      PRAGMA_UNROLL
-      for(int i = 0; i < items; ++i) {
-        float q = s.quarters(z[i]);
-        int b = sample_row_t::bin(q), down = top - b;
-        if(z[i] > -inf && down < sample_bins)
-          atomicAdd(&shared_table[down][lane], (unsigned)
-            (16777216.f * __builtin_amdgcn_exp2f(.25f * (q - b) - .25f)));
-      }
-      __syncthreads();
-      // Two threads a bin.
-      int bin = tid / 2;
-      float x = 0;
-      for(int i = 0; i < 32; ++i)
-        x += shared_table[bin][(tid & 1) * 32 + ((i + bin) & 31)];
-      x += dpp_move<dpp_quad_xor1>(x, x);
-      if(!(tid & 1)) mine.table[bin] = x * (1 / 16777216.f);
-    }
     sample_exp2_t exp2;
+    int top = sample_row_t::bin(s.quarters(m));
     double sum = 0;
     PRAGMA_UNROLL
     for(int c = 0; c < chunks; ++c) {
       double part = 0;
       PRAGMA_UNROLL
-      for(int i = c * W; i < c * W + W; ++i)
-        part += exp2(((double)z[i] - (double)m) * s.c);
+      for(int i = c * W; i < c * W + W; ++i) {
+        double e = exp2(((double)z[i] - (double)m) * s.c);
+        part += e;
+        if(!all) {
+          // In a measure of the bin's octave, so that 24 bits do: no column
+          // gets past 128 * 2^24.
+          int down = top - sample_row_t::bin(s.quarters(z[i]));
+          if(down < sample_bins)
+            atomicAdd(&shared_table[down][lane], (unsigned)
+              __builtin_amdgcn_ldexpf((float)e, 23 + (down >> 2)));
+        }
+      }
       if(all) {
         part = wave_allreduce(part, plus_t<double>(), lane);
         if(!lane) mine.segments[c * waves + tid / 64] = part;
@@ -327,17 +364,25 @@ struct sample_piece_f {
       for(int w = 1; w < waves; ++w) sum += shared_sum[w];
       mine.sum = sum;
     }
+    if(!all) {
+      float x = add_columns();
+      if(!(tid & 1))
+        mine.table[bin] = __builtin_amdgcn_ldexpf(x, -23 - (bin >> 2));
+    }
   }
 };
 
-// Probabilities as whole numbers.
+// Probabilities as whole numbers: adding 2^52 rounds to one.
 struct sample_scale_t {
-  int scale;
+  int scale;                    // at most 50
   __forceinline__ MGPU_DEVICE double one() const {
     return (double)(1ull << scale);
   }
   __forceinline__ MGPU_DEVICE mass_t whole(double share) const {
-    return (mass_t)(share * one() + .5);
+    double x = __builtin_fma(share, one(), 4503599627370496.);
+    mass_t bits;
+    __builtin_memcpy(&bits, &x, 8);
+    return bits - 0x4330000000000000ull;
   }
   // Octaves below the largest logit at which no probability is left.
   __forceinline__ MGPU_DEVICE int nothing_left() const { return scale + 2; }
@@ -398,12 +443,14 @@ struct sample_weigh_f {
       sum = wave_allreduce(sum, plus_t<double>(), lane);
       if(!lane) shared_sum[wave] = sum;
       float x = 0;
+      _Pragma("unroll 8")
       for(int p = 0; p < pieces; ++p) {
-        int b = tid - (top - sample_row_t::bin(s.quarters(of_row[p].max)));
-        if(b >= 0 && b < sample_bins) x += of_row[p].table[b];
+        float max = of_row[p].max;
+        int b = tid - (top - sample_row_t::bin(s.quarters(max)));
+        float part = of_row[p].table[min(mgpu::max(b, 0), sample_bins - 1)];
+        if(b >= 0 && b < sample_bins && max > -inf)
+          x += part * __builtin_amdgcn_exp2f(.5f * s.c2 * (max - m));
       }
-      // The top of bin tid, relative to the largest logit.
-      x *= __builtin_amdgcn_exp2f(.25f * (top + 1 - tid - q));
       float upto = wave_scan(x, plus_t<float>(), lane);
       if(63 == lane) shared_scan[wave] = upto;
       __syncthreads();
@@ -412,7 +459,7 @@ struct sample_weigh_f {
       for(int w = 1; w < waves; ++w) sum += shared_sum[w];
       for(int w = 0; w < wave; ++w) upto += shared_scan[w];
       float want = (float)(s.p * sum);
-      float margin = 1.0001f + 1e-6f * pieces + 4e-8f * far;
+      float margin = 1.0001f + 1e-6f * pieces;
       int less = popc(ballot(upto * margin < want));
       int reached = popc(ballot(upto < want * margin));
       if(!lane) {
@@ -428,8 +475,8 @@ struct sample_weigh_f {
       }
       // A piece's table ends after sample_bins bins; further down the sums are
       // not all there.
-      low = margin < 2 ? min(less, sample_bins - 1) : 0;
-      if(margin < 2 && reached < sample_bins) high = min(high, reached);
+      low = min(less, sample_bins - 1);
+      if(reached < sample_bins) high = min(high, reached);
     }
 
     unsigned in = 0;
@@ -444,11 +491,15 @@ struct sample_weigh_f {
         if(down < low) {
           double e = exp2(((double)z[i] - (double)m) * s.c);
           mass_t w = scale.whole(e);
-          above += w;
-          run += e >= s.least || z[i] == m ? w : 0;
+          if(s.least > 0) {
+            above += w;
+            run += e >= s.least || z[i] == m ? w : 0;
+          } else
+            run += w;
         } else
           in |= 1u << i;
       }
+      if(!(s.least > 0)) above += run;
       run = wave_allreduce(run, plus_t<mass_t>(), lane);
       if(!lane) mine.runs[c * waves + wave] = run;
     }
@@ -468,7 +519,7 @@ struct sample_weigh_f {
 // temperature at which all are nearly equal), it reads the row again: a border
 // is bracketed by the counts per half octave, the tokens above the bracket are
 // added up, those inside are listed, and the border is found among them.
-enum { sample_nt = 1024, sample_candidates = 16384, sample_row_bins = 128 };
+enum { sample_nt = 1024, sample_row_bins = 128 };
 
 // Which tokens are kept: those with a larger key, and of those with this one
 // the ones up to `last`.
@@ -503,7 +554,6 @@ struct sample_row_f {
     int index[sample_candidates];
     union {
       mass_t hist[nt];
-      int offsets[nt];
       struct {
         float most[sample_row_bins];  // upper bounds of mass
         int count[sample_row_bins];
@@ -670,32 +720,52 @@ struct sample_row_f {
     return max((mass_t)ceil(x), (mass_t)1);
   }
 
-  // The pieces' lists, one after the other.
-  __forceinline__ MGPU_DEVICE int gather_lists(const at_t& a, shared_t& shared) const {
-    int base = 0, tid = a.tid;
-    bool too_many = false;
-    for(int p0 = 0; p0 < pieces; p0 += nt) {
-      int mine = p0 + tid < pieces ? a.piece[p0 + tid].listed : 0;
-      too_many |= mine > sample_list;
-      int upto = scan(min(mine, (int)sample_list), tid, shared.wave_int);
-      __syncthreads();
-      shared.offsets[tid] = upto;
-      if(__syncthreads_or(too_many || base + upto > sample_candidates))
-        return sample_candidates + 1;
-      int here = min(pieces - p0, (int)nt);
-      for(int p = tid / 64; p < here; p += num_waves) {
-        int first = p ? shared.offsets[p - 1] : 0;
-        int count = shared.offsets[p] - first;
-        for(int i = tid & 63; i < count; i += 64) {
-          int v = (p0 + p) * sample_piece + a.piece[p0 + p].list[i];
-          shared.index[base + first + i] = v;
-          shared.key[base + first + i] = sample_key((float)a.z[v]);
+  // The pieces' lists, without what lies further down than the row's k-th
+  // token does by the pieces' counts.  More than sample_candidates: not all.
+  __forceinline__ MGPU_DEVICE int gather_lists(const at_t& a, shared_t& shared)
+    const {
+    int tid = a.tid, top = sample_key_bin(sample_key(a.m)), less = 0;
+    bool some = a.s.by_count && a.s.counted(pieces);
+    if(some) {
+      float x = 0;
+      if(tid < sample_bins)
+        for(int p = 0; p < pieces; ++p) {
+          float max = a.piece[p].max;
+          int b = tid - (top - sample_key_bin(sample_key(max)));
+          if(b >= 0 && max > -__builtin_inff()) x += a.piece[p].table[b];
+        }
+      float upto = scan(x, tid, shared.wave_float);
+      less = __syncthreads_count(tid < sample_bins && upto < a.s.k);
+    }
+    some = some && less < sample_bins;
+    if(!tid) shared.listed = 0;
+    __syncthreads();
+    for(int p = tid / 64; p < pieces; p += num_waves) {
+      int count = a.piece[p].listed;
+      if(count > sample_list) {
+        if(!(tid & 63)) atomicAdd(&shared.listed, (int)sample_candidates + 1);
+        break;
+      }
+      for(int i = tid & 63; i - (tid & 63) < count; i += 64) {
+        int v = 0;
+        unsigned key = 0;
+        if(i < count) {
+          v = p * sample_piece + a.piece[p].list[i];
+          key = sample_key((float)a.z[v]);
+        }
+        bool in = i < count && (!some || top - sample_key_bin(key) <= less);
+        lanemask_t mask = ballot(in);
+        int base = 0;
+        if(!(tid & 63) && mask) base = atomicAdd(&shared.listed, popc(mask));
+        int at = readlane(base, 0) + popc(mask & lanemask_lt(tid & 63));
+        if(in && at < sample_candidates) {
+          shared.key[at] = key;
+          shared.index[at] = v;
         }
       }
-      base += shared.offsets[here - 1];
-      __syncthreads();
     }
-    return base;
+    __syncthreads();
+    return shared.listed;
   }
 
   // use(v, chunks): 16 tokens of every thread at a time; chunk c begins at
@@ -1259,7 +1329,11 @@ void sample_launch(const type_t* logits, int64_t stride, int rows, int vocab,
   sample_scale_t scale { min(62 - bits, 50) };
   sample_weigh_f<type_t> weigh { logits, stride, vocab, pieces, scale, settings,
     from };
-  cta_launch<sample_piece_nt>(weigh, rows * pieces, context);
+  // Not where all rows are known to have top-k, or neither top-p nor min-p.
+  if((settings.top_k || settings.top_k_all <= 0 || settings.top_k_all >= vocab) &&
+    (settings.top_p || settings.top_p_all < 1 || settings.min_p ||
+      settings.min_p_all > 0))
+    cta_launch<sample_piece_nt>(weigh, rows * pieces, context);
   sample_row_f<type_t> draw { logits, stride, vocab, pieces, scale, uniform,
     settings, from, token, logprob };
   cta_launch<sample_nt>(draw, rows, context);
