@@ -417,8 +417,6 @@ struct sample_weigh_f {
     if(s.by_count || s.all()) return;
     sample_piece_t& mine = out[cta];
     const sample_piece_t* of_row = out + (int64_t)row * pieces;
-    tokens_t tokens(logits + row * stride, piece, vocab, tid);
-    const float (&z)[items] = tokens.z;
 
     float m = -inf;
     for(int p = tid; p < pieces; p += nt) m = __builtin_fmaxf(m, of_row[p].max);
@@ -433,7 +431,8 @@ struct sample_weigh_f {
     float q = s.quarters(m), far = __builtin_fabsf(q) + 4 * sample_bins;
     int top = sample_row_t::bin(q), slack = 1 + (int)(3e-7f * far);
     int low = 0x7fffffff, high = 4 * scale.nothing_left();
-    if(s.least > 0) high = min(high, (int)(-4 * (float)log2(s.least)));
+    if(s.least > 0)
+      high = min(high, (int)(-4 * __builtin_amdgcn_logf((float)s.least)));
     high += slack;
     if(s.by_mass) {
       double sum = 0;
@@ -443,13 +442,25 @@ struct sample_weigh_f {
       sum = wave_allreduce(sum, plus_t<double>(), lane);
       if(!lane) shared_sum[wave] = sum;
       float x = 0;
-      _Pragma("unroll 8")
-      for(int p = 0; p < pieces; ++p) {
-        float max = of_row[p].max;
-        int b = tid - (top - sample_row_t::bin(s.quarters(max)));
-        float part = of_row[p].table[min(mgpu::max(b, 0), sample_bins - 1)];
-        if(b >= 0 && b < sample_bins && max > -inf)
-          x += part * __builtin_amdgcn_exp2f(.5f * s.c2 * (max - m));
+      for(int p0 = 0; p0 < pieces; p0 += 64) {
+        // Lane p has a piece's place in the row's bins and its measure.
+        int off = 0;
+        float measure = 0;
+        if(p0 + lane < pieces) {
+          float max = of_row[p0 + lane].max;
+          off = top - sample_row_t::bin(s.quarters(max));
+          if(max > -inf)
+            measure = __builtin_amdgcn_exp2f(.5f * s.c2 * (max - m));
+        }
+        int count = min(pieces - p0, 64);
+        _Pragma("unroll 8")
+        for(int p = 0; p < count; ++p) {
+          int b = tid - readlane(off, p);
+          float by = readlane(measure, p);
+          float part = of_row[p0 + p].table[min(mgpu::max(b, 0),
+            sample_bins - 1)];
+          x += b == (b & (sample_bins - 1)) ? part * by : 0.f;
+        }
       }
       float upto = wave_scan(x, plus_t<float>(), lane);
       if(63 == lane) shared_scan[wave] = upto;
@@ -479,11 +490,31 @@ struct sample_weigh_f {
       if(reached < sample_bins) high = min(high, reached);
     }
 
+    // No logit below this is in a bin up to `high`: most pieces and runs of a
+    // peaked row have none, and are passed over.
+    float floor = m - (high + 1 + slack) / (2 * s.c2);
+    if(mine.max < floor) {
+      if(tid < sample_segments) mine.runs[tid] = 0;
+      if(!tid) {
+        mine.above = 0;
+        mine.listed = 0;
+      }
+      return;
+    }
+    tokens_t tokens(logits + row * stride, piece, vocab, tid);
+    const float (&z)[items] = tokens.z;
     unsigned in = 0;
     mass_t above = 0;
     PRAGMA_UNROLL
     for(int c = 0; c < chunks; ++c) {
       mass_t run = 0;
+      float most = z[c * W];
+      PRAGMA_UNROLL
+      for(int i = 1; i < W; ++i) most = __builtin_fmaxf(most, z[c * W + i]);
+      if(!ballot(!(most < floor))) {
+        if(!lane) mine.runs[c * waves + wave] = 0;
+        continue;
+      }
       PRAGMA_UNROLL
       for(int i = c * W; i < c * W + W; ++i) {
         int down = top - sample_row_t::bin(s.quarters(z[i]));
@@ -699,7 +730,8 @@ struct sample_row_f {
     // Nothing further down is drawn.
     float reach = nothing_left();
     if(a.s.least > 0)
-      reach = __builtin_fminf(reach, .01f - 2 * (float)log2(a.s.least));
+      reach = __builtin_fminf(reach, .01f -
+        2 * __builtin_amdgcn_logf((float)a.s.least));
     bool lists = !a.s.by_count || a.s.k <= sample_max_k;
     int n = lists ? gather_lists(a, shared) : 0;
     lists = lists && n <= sample_candidates;
