@@ -24,11 +24,21 @@ enum { distill_max_top = 1024 };
 
 namespace detail {
 
-enum { distill_nt = 512 };
 enum distill_mode_t { distill_loss_only, distill_grad_only, distill_both };
 
-template<typename type_t, typename teacher_t, distill_mode_t mode>
+// One CTA per row.  With chunks > 0 the row stays in registers, `chunks` 16-byte
+// pieces a thread, between the pass that sums it and the pass that writes the
+// gradient: it is read once.  The loads are all in flight while the teacher's
+// entries are dealt with.  With chunks == 0 (longer rows, and where only one
+// of the two passes is made) the row is walked.
+template<typename type_t, typename teacher_t, distill_mode_t mode, int nt_,
+  int chunks>
 struct distill_f {
+  enum { nt = nt_, waves = nt / 64, W = row_chunk_t<type_t>::width,
+    entries = distill_max_top / nt, slots = 4096 };
+  typedef row_chunk_t<type_t> chunk_t;
+  typedef row_held_t<type_t> held_t;
+
   const type_t* logits;
   int64_t stride;
   int vocab;
@@ -42,32 +52,118 @@ struct distill_f {
   type_t* grad;
   int64_t grad_stride;
 
-  MGPU_DEVICE void operator()(int tid, int row) const {
-    enum { nt = distill_nt, W = row_chunk_t<type_t>::width };
-    typedef row_chunk_t<type_t> chunk_t;
+  // 2^((x - m) c).  The difference first: it is exact where it matters, and
+  // m c may lie past the largest float.
+  __forceinline__ MGPU_DEVICE float share(float x, float m) const {
+    return __builtin_amdgcn_exp2f((x - m) * c);
+  }
+
+  // Adds a chunk to a running largest logit and sum of shares of it.
+  __forceinline__ MGPU_DEVICE void add(const held_t& ch, float& m, float& s)
+    const {
+    const float inf = __builtin_inff();
+    float y = m;
+    PRAGMA_UNROLL
+    for(int i = 0; i < W; ++i) y = __builtin_fmaxf(y, ch.get(i));
+    if(y != m) s *= share(m, y);
+    m = y;
+    // -inf all through so far, or NaN: differences from 0 then.
+    float from = m == -inf ? 0.f : m;
+    PRAGMA_UNROLL
+    for(int i = 0; i < W; ++i) s += share(ch.get(i), from);
+  }
+
+  // The sum of s over the CTA, measured from the largest m, which m becomes.
+  __forceinline__ MGPU_DEVICE float join(float& m, float s, int tid,
+    float (&shared)[2][waves]) const {
+    const float inf = __builtin_inff();
+    float all = wave_allreduce(m, float_max_t(), tid & 63);
+    if(m != all && m != -inf) s *= share(m, all);
+    s = wave_allreduce(s, plus_t<float>(), tid & 63);
+    if(!(tid & 63)) {
+      shared[0][tid / 64] = all;
+      shared[1][tid / 64] = s;
+    }
+    __syncthreads();
+    m = shared[0][0];
+    PRAGMA_UNROLL
+    for(int w = 1; w < waves; ++w) m = __builtin_fmaxf(m, shared[0][w]);
+    s = 0;
+    PRAGMA_UNROLL
+    for(int w = 0; w < waves; ++w) {
+      float x = shared[0][w], y = shared[1][w];
+      s += x != m && x != -inf ? y * share(x, m) : y;
+    }
+    return s;
+  }
+
+  __forceinline__ MGPU_DEVICE void write(const held_t& ch, type_t* dz, int v,
+    float m, float scale) const {
+    float x[W];
+    PRAGMA_UNROLL
+    for(int i = 0; i < W; ++i) x[i] = scale * share(ch.get(i), m);
+    row_store(x, dz + v, vocab - v);
+  }
+
+  __forceinline__ MGPU_DEVICE void operator()(int tid, int row) const {
     const float inf = __builtin_inff();
     const float ln2 = 0.693147180559945309f;
-    __shared__ float shared_p[distill_max_top];
+    __shared__ float shared_a[distill_max_top];
     __shared__ int shared_id[distill_max_top];
-    __shared__ float shared_reduce[5][nt / 64];
+    __shared__ unsigned short shared_slot[slots];
+    __shared__ bool shared_twice[distill_max_top];
+    __shared__ float shared_join[2][2][waves], shared_reduce[waves];
 
     const type_t* z = logits + row * stride;
     type_t* dz = grad + row * grad_stride;
     float w = weights ? weights[row] : 1.f;
+    bool live = w != 0;
 
-    // The teacher's softmax.
-    float a_max = -inf;
-    if(w != 0)
-      for(int k = tid; k < top; k += nt) {
-        int id = ids[(int64_t)row * top + k];
-        bool ok = (unsigned)id < (unsigned)vocab;
-        float a = ok ? (float)teacher[(int64_t)row * top + k] : -inf;
-        shared_id[k] = ok ? id : -1;
-        shared_p[k] = a;
-        a_max = __builtin_fmaxf(a_max, a != a ? inf : a);
+    // The teacher's entries of this thread.
+    int id[entries];
+    float a[entries];
+    PRAGMA_UNROLL
+    for(int j = 0; j < entries; ++j) {
+      int k = tid + j * nt;
+      id[j] = -1;
+      a[j] = -inf;
+      if(live && k < top) {
+        id[j] = ids[(int64_t)row * top + k];
+        a[j] = (float)teacher[(int64_t)row * top + k];
       }
-    a_max = cta_allreduce<nt>(a_max, float_max_t(), tid, shared_reduce[0]);
-    if(w == 0 || a_max == -inf) {
+    }
+    held_t held[chunks ? chunks : 1];
+    if(chunks && live) {
+      PRAGMA_UNROLL
+      for(int i = 0; i < chunks; ++i) {
+        int v = (i * nt + tid) * W;
+        held[i].load(z + v, vocab - v, (type_t)-inf);
+      }
+    }
+    float at[entries];            // the logits at the entries' indices
+    float a_max = -inf, a_sum = 0;
+    PRAGMA_UNROLL
+    for(int j = 0; j < entries; ++j) {
+      if((unsigned)id[j] >= (unsigned)vocab) {
+        id[j] = -1;
+        a[j] = -inf;
+      }
+      at[j] = id[j] >= 0 ? (float)z[id[j]] : 0.f;
+      // NaN goes on as an infinite maximum.
+      a_max = __builtin_fmaxf(a_max, a[j] != a[j] ? inf : a[j]);
+      int k = tid + j * nt;
+      if(k < top) {
+        shared_id[k] = id[j];
+        shared_a[k] = a[j];
+        shared_twice[k] = false;
+        if(id[j] >= 0) shared_slot[id[j] % slots] = (unsigned short)k;
+      }
+    }
+    PRAGMA_UNROLL
+    for(int j = 0; j < entries; ++j)
+      if(id[j] >= 0 && a_max != -inf) a_sum += share(a[j], a_max);
+    a_sum = join(a_max, a_sum, tid, shared_join[0]);
+    if(a_max == -inf) {
       if(!tid && loss) loss[row] = 0;
       if(!tid && norms) norms[2 * (int64_t)row] = norms[2 * (int64_t)row + 1] = 0;
       if(mode != distill_loss_only) {
@@ -79,12 +175,44 @@ struct distill_f {
       }
       return;
     }
-    float a_sum = 0;
-    for(int k = tid; k < top; k += nt) {
-      float p = __builtin_amdgcn_exp2f((shared_p[k] - a_max) * c);
-      a_sum += p;
+
+    // Entries that share an index: of those in one slot, all but the one that
+    // got it look through the others, and so does that one if it is among
+    // those with its index.
+    bool look[entries];
+    if(mode != distill_loss_only) {
+      PRAGMA_UNROLL
+      for(int j = 0; j < entries; ++j) {
+        int k = tid + j * nt;
+        look[j] = false;
+        if(id[j] >= 0) {
+          int other = shared_slot[id[j] % slots];
+          look[j] = other != k;
+          if(look[j] && shared_id[other] == id[j]) shared_twice[other] = true;
+        }
+      }
+      __syncthreads();
     }
-    a_sum = cta_allreduce<nt>(a_sum, plus_t<float>(), tid, shared_reduce[1]);
+    float inv_a = 1 / a_sum, log2_a = __builtin_amdgcn_logf(a_sum);
+    float p[entries], total[entries];
+    PRAGMA_UNROLL
+    for(int j = 0; j < entries; ++j) {
+      int k = tid + j * nt;
+      p[j] = id[j] >= 0 ? share(a[j], a_max) * inv_a : 0.f;
+      total[j] = p[j];
+      if(mode != distill_loss_only && id[j] >= 0 && (look[j] || shared_twice[k])) {
+        // The first of the entries with this index stands for all.
+        float sum = 0;
+        bool first = true;
+        for(int i = 0; i < top; ++i)
+          if(shared_id[i] == id[j]) {
+            first &= i >= k;
+            sum += share(shared_a[i], a_max);
+          }
+        total[j] = sum * inv_a;
+        if(!first) id[j] = ~id[j];
+      }
+    }
 
     // The row's maximum and sum.
     float m, log2_s;
@@ -92,93 +220,82 @@ struct distill_f {
       m = norms[2 * (int64_t)row];
       log2_s = norms[2 * (int64_t)row + 1] / ln2;
     } else {
-      float x = -inf, s = 0;
-      for(int v = tid * W; v < vocab; v += nt * W) {
-        chunk_t ch;
-        ch.load(z + v, vocab - v, (type_t)-inf);
-        float y = x;
+      float s = 0;
+      m = -inf;
+      if(chunks) {
         PRAGMA_UNROLL
-        for(int i = 0; i < W; ++i) y = __builtin_fmaxf(y, (float)ch.x[i]);
-        if(y != x) s *= __builtin_amdgcn_exp2f((x - y) * c);
-        x = y;
-        if(x != -inf) {
+        for(int i = 0; i < chunks; ++i) {
           PRAGMA_UNROLL
-          for(int i = 0; i < W; ++i)
-            s += __builtin_amdgcn_exp2f(((float)ch.x[i] - x) * c);
-        } else {
-          // -inf all through, or NaN
+          for(int j = 0; j < W; ++j)
+            m = __builtin_fmaxf(m, held[i].get(j));
+        }
+        float from = m == -inf ? 0.f : m;
+        PRAGMA_UNROLL
+        for(int i = 0; i < chunks; ++i) {
+          held[i].renew();
           PRAGMA_UNROLL
-          for(int i = 0; i < W; ++i)
-            if(ch.x[i] != ch.x[i]) s = (float)ch.x[i];
+          for(int j = 0; j < W; ++j) s += share(held[i].get(j), from);
+        }
+      } else {
+        for(int v = tid * W; v < vocab; v += nt * W) {
+          held_t ch;
+          ch.load(z + v, vocab - v, (type_t)-inf);
+          add(ch, m, s);
         }
       }
-      m = cta_allreduce<nt>(x, float_max_t(), tid, shared_reduce[2]);
-      if(x != m) s = x == -inf ? s : s * __builtin_amdgcn_exp2f((x - m) * c);
-      s = cta_allreduce<nt>(s, plus_t<float>(), tid, shared_reduce[3]);
+      s = join(m, s, tid, shared_join[1]);
       log2_s = __builtin_amdgcn_logf(s);
     }
     bool none = m == -inf && log2_s == -inf;    // with a NaN, log2_s is NaN
+    float from = none ? 0.f : m;
     float inv_s = none ? 0.f : __builtin_amdgcn_exp2f(-log2_s);
 
-    // The entries: loss terms, and what each adds to its column.
-    float inv_a = 1 / a_sum, log2_a = __builtin_amdgcn_logf(a_sum);
-    float coef = w * tau, sum = 0;
-    float entry[(distill_max_top + nt - 1) / nt];
-    int column[(distill_max_top + nt - 1) / nt];
+    // The entries' loss terms, and what stands in their columns.
+    float coef = w * tau, sum = 0, column[entries];
     PRAGMA_UNROLL
-    for(int j = 0; j < (distill_max_top + nt - 1) / nt; ++j) {
-      int k = tid + j * nt;
-      column[j] = -1;
-      if(k < top && shared_id[k] >= 0) {
-        int id = shared_id[k];
-        float d = (shared_p[k] - a_max) * c;
-        float p = __builtin_amdgcn_exp2f(d) * inv_a;
-        float y = none ? -inf : ((float)z[id] - m) * c;
-        if(mode != distill_grad_only && !(p == 0))
-          sum += p * ((d - log2_a) - (none ? y : y - log2_s)) * ln2;
-        if(mode != distill_loss_only) {
-          // The first of the entries with this index stands for all.
-          float total = 0;
-          bool first = true;
-          for(int i = 0; i < top; ++i)
-            if(shared_id[i] == id) {
-              first &= i >= k;
-              total += __builtin_amdgcn_exp2f((shared_p[i] - a_max) * c);
-            }
-          if(first) column[j] = id;
-          float q = none ? 0.f : __builtin_amdgcn_exp2f(y) * inv_s;
-          entry[j] = coef * (q - total * inv_a);
-        }
+    for(int j = 0; j < entries; ++j) {
+      if(mode != distill_grad_only && !(p[j] == 0)) {
+        float log2_q = none ? -inf : (at[j] - m) * c - log2_s;
+        sum += p[j] * ((a[j] - a_max) * c - log2_a - log2_q) * ln2;
       }
+      column[j] = coef * (share(at[j], from) * inv_s - total[j]);
     }
     if(mode != distill_grad_only) {
-      sum = cta_allreduce<nt>(sum, plus_t<float>(), tid, shared_reduce[4]);
-      if(!tid) {
-        loss[row] = w * tau * tau * sum;
-        if(norms) {
-          norms[2 * (int64_t)row] = m;
-          norms[2 * (int64_t)row + 1] = log2_s * ln2;
-        }
+      sum = wave_allreduce(sum, plus_t<float>(), tid & 63);
+      if(!(tid & 63)) shared_reduce[tid / 64] = sum;
+    }
+    // (Every logit at an entry has been read before the first store: dz may
+    // be z.)
+    __syncthreads();
+    if(mode != distill_grad_only && !tid) {
+      PRAGMA_UNROLL
+      for(int i = 1; i < waves; ++i) sum += shared_reduce[i];
+      loss[row] = w * tau * tau * sum;
+      if(norms) {
+        norms[2 * (int64_t)row] = m;
+        norms[2 * (int64_t)row + 1] = log2_s * ln2;
       }
     }
     if(mode != distill_loss_only) {
-      // Every z[id] has been read before the first store (dz may be z).
-      __syncthreads();
-      for(int v = tid * W; v < vocab; v += nt * W) {
-        chunk_t ch;
-        ch.load(z + v, vocab - v, (type_t)0.f);
+      float scale = coef * inv_s;
+      if(chunks) {
         PRAGMA_UNROLL
-        for(int i = 0; i < W; ++i) {
-          float q = none ? 0.f :
-            __builtin_amdgcn_exp2f(((float)ch.x[i] - m) * c) * inv_s;
-          ch.x[i] = (type_t)(coef * q);
+        for(int i = 0; i < chunks; ++i) {
+          int v = (i * nt + tid) * W;
+          held[i].renew();
+          if(v < vocab) write(held[i], dz, v, from, scale);
         }
-        ch.store(dz + v, vocab - v);
+      } else {
+        for(int v = tid * W; v < vocab; v += nt * W) {
+          held_t ch;
+          ch.load(z + v, vocab - v, (type_t)-inf);
+          write(ch, dz, v, from, scale);
+        }
       }
       __syncthreads();
       PRAGMA_UNROLL
-      for(int j = 0; j < (distill_max_top + nt - 1) / nt; ++j)
-        if(column[j] >= 0) dz[column[j]] = (type_t)entry[j];
+      for(int j = 0; j < entries; ++j)
+        if(id[j] >= 0) dz[id[j]] = (type_t)column[j];
     }
   }
 };
@@ -189,10 +306,23 @@ void distill_launch(const type_t* logits, int64_t stride, int rows, int vocab,
   const float* weights, float* loss, float* norms, type_t* grad,
   int64_t grad_stride, context_t& context) {
   if(rows <= 0) return;
-  distill_f<type_t, teacher_t, mode> k { logits, stride, vocab, ids, teacher,
-    top, tau, (float)(1.4426950408889634 / tau), weights, loss, norms, grad,
-    grad_stride };
-  cta_launch<distill_nt>(k, rows, context);
+  auto launch = [&](auto k) {
+    typedef decltype(k) f_t;
+    f_t f { logits, stride, vocab, ids, teacher, top, tau,
+      (float)(1.4426950408889634 / tau), weights, loss, norms, grad,
+      grad_stride };
+    cta_launch<f_t::nt>(f, rows, context);
+  };
+  enum { W = row_chunk_t<type_t>::width };
+  if constexpr(mode == distill_both) {
+    if(vocab <= 256 * 4 * W)
+      return launch(distill_f<type_t, teacher_t, mode, 256, 4>());
+    if(vocab <= 512 * 8 * W)
+      return launch(distill_f<type_t, teacher_t, mode, 512, 8>());
+    if(vocab <= 1024 * 16 * W)
+      return launch(distill_f<type_t, teacher_t, mode, 1024, 16>());
+  }
+  launch(distill_f<type_t, teacher_t, mode, 512, 0>());
 }
 
 } // namespace detail

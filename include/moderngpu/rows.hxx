@@ -9,6 +9,7 @@
 // row is walked in 16-byte chunks counted from its own start, and only the
 // chunk that would cross the row's end goes value by value.
 #pragma once
+#include <type_traits>
 #include "intrinsics.hxx"
 #include "transform.hxx"
 
@@ -62,6 +63,60 @@ struct row_chunk_t {
     }
   }
 };
+
+// A chunk that stays as its four words and is taken apart where it is used:
+// 16-bit values that live long as separate ones would take twice the registers.
+template<typename type_t>
+struct row_held_t {
+  enum { width = 16 / sizeof(type_t) };
+  typedef row_words_at_t<sizeof(type_t)> any_words_t;
+  unsigned w[4];
+
+  __forceinline__ MGPU_DEVICE void load(const type_t* p, int n, type_t rest) {
+    row_words_t x;
+    if(n >= width) x = ((const any_words_t*)p)->w;
+    else {
+      row_chunk_t<type_t> ch;
+      ch.load(p, n, rest);
+      __builtin_memcpy(&x, ch.x, 16);
+    }
+    __builtin_memcpy(w, &x, 16);
+  }
+  __forceinline__ MGPU_DEVICE float get(int i) const {
+    if constexpr(std::is_same<type_t, bf16_t>::value)
+      return __builtin_bit_cast(float,
+        i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else if constexpr(2 == sizeof(type_t))
+      return (float)__builtin_bit_cast(type_t, (unsigned short)
+        (i & 1 ? w[i / 2] >> 16 : w[i / 2]));
+    else
+      return __builtin_bit_cast(float, w[i]);
+  }
+  // From here on the words count as new: nothing taken from them before is
+  // kept for later.
+  __forceinline__ MGPU_DEVICE void renew() {
+#ifdef __HIP_DEVICE_COMPILE__
+    asm("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
+#endif
+  }
+};
+
+// width floats, each rounded to the row's type, to n of its values at p.
+template<typename type_t>
+__forceinline__ MGPU_DEVICE void row_store(
+  const float (&x)[row_chunk_t<type_t>::width], type_t* p, int n) {
+  typedef float pair_t __attribute__((ext_vector_type(2)));
+  typedef type_t two_t __attribute__((ext_vector_type(2)));
+  row_chunk_t<type_t> ch;
+  PRAGMA_UNROLL
+  for(int i = 0; i < row_chunk_t<type_t>::width; i += 2) {
+    pair_t f = { x[i], x[i + 1] };
+    two_t t = __builtin_convertvector(f, two_t);
+    ch.x[i] = t.x;
+    ch.x[i + 1] = t.y;
+  }
+  ch.store(p, n);
+}
 
 // `width` values of a row, in 16-byte moves where they fill some: the results
 // for a chunk of inputs of a narrower type.
