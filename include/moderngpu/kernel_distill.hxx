@@ -26,11 +26,10 @@ namespace detail {
 
 enum distill_mode_t { distill_loss_only, distill_grad_only, distill_both };
 
-// One CTA per row.  With chunks > 0 the row stays in registers, `chunks` 16-byte
-// pieces a thread, between the pass that sums it and the pass that writes the
-// gradient: it is read once.  The loads are all in flight while the teacher's
-// entries are dealt with.  With chunks == 0 (longer rows, and where only one
-// of the two passes is made) the row is walked.
+// One CTA per row.  The row's front, `chunks` 16-byte pieces a thread, stays in
+// registers between the pass that sums it and the pass that writes the
+// gradient, and is read once; its loads are all in flight while the teacher's
+// entries are dealt with.  What a longer row has behind that is read by both.
 template<typename type_t, typename teacher_t, distill_mode_t mode, int nt_,
   int chunks>
 struct distill_f {
@@ -103,6 +102,27 @@ struct distill_f {
     PRAGMA_UNROLL
     for(int i = 0; i < W; ++i) x[i] = scale * share(ch.get(i), m);
     row_store(x, dz + v, vocab - v);
+  }
+
+  // What of the row is not held, four chunks of the thread at a time.
+  template<typename use_t>
+  __forceinline__ MGPU_DEVICE void walk(const type_t* z, int tid, use_t use)
+    const {
+    const float inf = __builtin_inff();
+    PRAGMA_NO_UNROLL
+    for(int v0 = chunks * nt * W; v0 < vocab; v0 += 4 * nt * W) {
+      held_t ch[4];
+      PRAGMA_UNROLL
+      for(int i = 0; i < 4; ++i) {
+        int v = v0 + (i * nt + tid) * W;
+        ch[i].load(z + v, vocab - v, (type_t)-inf);
+      }
+      PRAGMA_UNROLL
+      for(int i = 0; i < 4; ++i) {
+        int v = v0 + (i * nt + tid) * W;
+        if(v < vocab) use(ch[i], v);
+      }
+    }
   }
 
   __forceinline__ MGPU_DEVICE void operator()(int tid, int row) const {
@@ -222,27 +242,19 @@ struct distill_f {
     } else {
       float s = 0;
       m = -inf;
-      if(chunks) {
+      PRAGMA_UNROLL
+      for(int i = 0; i < chunks; ++i) {
         PRAGMA_UNROLL
-        for(int i = 0; i < chunks; ++i) {
-          PRAGMA_UNROLL
-          for(int j = 0; j < W; ++j)
-            m = __builtin_fmaxf(m, held[i].get(j));
-        }
-        float from = m == -inf ? 0.f : m;
-        PRAGMA_UNROLL
-        for(int i = 0; i < chunks; ++i) {
-          held[i].renew();
-          PRAGMA_UNROLL
-          for(int j = 0; j < W; ++j) s += share(held[i].get(j), from);
-        }
-      } else {
-        for(int v = tid * W; v < vocab; v += nt * W) {
-          held_t ch;
-          ch.load(z + v, vocab - v, (type_t)-inf);
-          add(ch, m, s);
-        }
+        for(int j = 0; j < W; ++j) m = __builtin_fmaxf(m, held[i].get(j));
       }
+      float from = m == -inf ? 0.f : m;
+      PRAGMA_UNROLL
+      for(int i = 0; i < chunks; ++i) {
+        held[i].renew();
+        PRAGMA_UNROLL
+        for(int j = 0; j < W; ++j) s += share(held[i].get(j), from);
+      }
+      walk(z, tid, [&](const held_t& ch, int) { add(ch, m, s); });
       s = join(m, s, tid, shared_join[1]);
       log2_s = __builtin_amdgcn_logf(s);
     }
@@ -278,20 +290,13 @@ struct distill_f {
     }
     if(mode != distill_loss_only) {
       float scale = coef * inv_s;
-      if(chunks) {
-        PRAGMA_UNROLL
-        for(int i = 0; i < chunks; ++i) {
-          int v = (i * nt + tid) * W;
-          held[i].renew();
-          if(v < vocab) write(held[i], dz, v, from, scale);
-        }
-      } else {
-        for(int v = tid * W; v < vocab; v += nt * W) {
-          held_t ch;
-          ch.load(z + v, vocab - v, (type_t)-inf);
-          write(ch, dz, v, from, scale);
-        }
+      PRAGMA_UNROLL
+      for(int i = 0; i < chunks; ++i) {
+        int v = (i * nt + tid) * W;
+        held[i].renew();
+        if(v < vocab) write(held[i], dz, v, from, scale);
       }
+      walk(z, tid, [&](const held_t& ch, int v) { write(ch, dz, v, from, scale); });
       __syncthreads();
       PRAGMA_UNROLL
       for(int j = 0; j < entries; ++j)
@@ -315,14 +320,21 @@ void distill_launch(const type_t* logits, int64_t stride, int rows, int vocab,
   };
   enum { W = row_chunk_t<type_t>::width };
   if constexpr(mode == distill_both) {
+    // As few threads as hold the row, so that several rows are on their way
+    // on a CU.  Past 32768 16-bit values that is one row in all its registers,
+    // and two rows of which each holds half are faster (2048 x 65536 bf16: 114
+    // us against 191 with 1024 threads, x 131072: 242 against 280; two that
+    // hold a quarter: 121 and 272).  32-bit rows have half the arithmetic a
+    // byte, and one row held by 1024 threads does (1024 x 65536: 128 us
+    // against 133, x 131072: 254 against 289).
     if(vocab <= 256 * 4 * W)
       return launch(distill_f<type_t, teacher_t, mode, 256, 4>());
     if(vocab <= 512 * 8 * W)
       return launch(distill_f<type_t, teacher_t, mode, 512, 8>());
-    if(vocab <= 1024 * 16 * W)
-      return launch(distill_f<type_t, teacher_t, mode, 1024, 16>());
-  }
-  launch(distill_f<type_t, teacher_t, mode, 512, 0>());
+    return launch(distill_f<type_t, teacher_t, mode,
+      2 == sizeof(type_t) ? 512 : 1024, 16>());
+  } else
+    launch(distill_f<type_t, teacher_t, mode, 512, 0>());
 }
 
 } // namespace detail

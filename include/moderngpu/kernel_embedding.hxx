@@ -22,7 +22,7 @@ struct embedding_shape_t {
   int col_blocks;       // CTAs along a row
   embedding_shape_t(int dim, int width) {
     int chunks = div_up(dim, width);
-    cols = 1;
+    cols = 8;
     while(cols < chunks && cols < embedding_nt) cols *= 2;
     rows = embedding_nt / cols;
     col_blocks = div_up(chunks, cols);
@@ -82,50 +82,60 @@ enum { embedding_plan_nt = 1024, embedding_plan_rows = 512,
 // put in order by a counting sort.  Every wave has a contiguous piece of the
 // tokens and counters of its own, so equal ids keep their token order.  T ids
 // are read (rows / embedding_plan_rows) times, from L2; a radix sort would
-// read them less often but takes six dependent launches for 17-bit ids.
+// read them less often but takes six dependent launches for 17-bit ids.  Up to
+// 16384 tokens stay in registers between the two passes.
 struct embedding_plan_f {
+  enum { nt = embedding_plan_nt, R = embedding_plan_rows, W = nt / 64,
+    rounds = 16 };
   const int* ids;
   int count, num_rows;
   int* starts;                  // num_rows + 1
   int* order;                   // count
 
+  // The wave's ids at t + 64 * u + lane, u < rounds; -1 past the end.
+  __forceinline__ MGPU_DEVICE void load(int t, int end, int lane,
+    int (&id)[rounds]) const {
+    PRAGMA_UNROLL
+    for(int u = 0; u < rounds; ++u) {
+      int i = t + 64 * u + lane;
+      id[u] = i < end ? ids[i] : -1;
+    }
+  }
+
   MGPU_DEVICE void operator()(int tid, int cta) const {
-    enum { nt = embedding_plan_nt, R = embedding_plan_rows, W = nt / 64,
-      unroll = 8 };
     __shared__ int counters[W][R];
     __shared__ int shared_int[W], shared_scan[W];
     int wave = tid / 64, lane = tid & 63;
     int v0 = cta * R;
     int rows = min((int)R, num_rows - v0);
 
+    // The wave's tokens (count < 2^30, see embedding_grid_ok).
+    int piece = div_up(div_up(count, (int)W), 64) * 64;
+    int begin = (int)min(wave * (int64_t)piece, (int64_t)count);
+    int end = (int)min(begin + (int64_t)piece, (int64_t)count);
+    int id[rounds];
+    load(begin, end, lane, id);
+
     for(int i = tid; i < W * R; i += nt) (&counters[0][0])[i] = 0;
     __syncthreads();
-
-    // The wave's tokens, 64 at a time; T < 2^31 - 2^20 (see the launch).
-    int piece = div_up(div_up(count, (int)W), 64) * 64;
-    int begin = min(wave * (int64_t)piece, (int64_t)count);
-    int end = min(begin + (int64_t)piece, (int64_t)count);
     int less = 0;
-    for(int t = begin; t < end; t += 64 * unroll) {
-      int id[unroll];
+    for(int t = begin; t < end; t += 64 * rounds) {
+      if(t > begin) load(t, end, lane, id);
       PRAGMA_UNROLL
-      for(int u = 0; u < unroll; ++u) {
-        int i = t + 64 * u + lane;
-        id[u] = i < end ? ids[i] : -1;
-      }
-      PRAGMA_UNROLL
-      for(int u = 0; u < unroll; ++u) {
-        int r = id[u] - v0;
+      for(int u = 0; u < rounds; ++u) {
         less += id[u] >= 0 && id[u] < v0;
-        if(id[u] >= v0 && r < rows) atomicAdd(&counters[wave][r], 1);
+        if(id[u] >= v0 && id[u] - v0 < rows)
+          atomicAdd(&counters[wave][id[u] - v0], 1);
       }
     }
     less = cta_allreduce<nt>(less, plus_t<int>(), tid, shared_int);
 
     // Where each wave's tokens of each row go.
     int total = 0;
-    if(tid < rows)
+    if(tid < rows) {
+      PRAGMA_UNROLL
       for(int w = 0; w < W; ++w) total += counters[w][tid];
+    }
     int upto = wave_scan(total, plus_t<int>(), lane);
     if(63 == lane) shared_scan[wave] = upto;
     __syncthreads();
@@ -142,25 +152,25 @@ struct embedding_plan_f {
     }
     __syncthreads();
 
-    for(int t = begin; t < end; t += 64 * unroll) {
-      int id[unroll];
+    for(int t = begin; t < end; t += 64 * rounds) {
+      if(end - begin > 64 * rounds) load(t, end, lane, id);
       PRAGMA_UNROLL
-      for(int u = 0; u < unroll; ++u) {
-        int i = t + 64 * u + lane;
-        id[u] = i < end ? ids[i] : -1;
-      }
-      PRAGMA_UNROLL
-      for(int u = 0; u < unroll; ++u) {
+      for(int u = 0; u < rounds; ++u) {
         int r = id[u] - v0;
         bool mine = id[u] >= v0 && r < rows;
         lanemask_t peers = ballot(mine);
         if(!peers) continue;
-        for(int b = 1; b < R; b *= 2) {
-          lanemask_t set = ballot(r & b);
-          peers &= r & b ? set : ~set;
+        if(peers & (peers - 1)) {
+          // More than one: those with the same row.
+          PRAGMA_NO_UNROLL
+          for(int b = 1; b < R; b *= 2) {
+            lanemask_t set = ballot(r & b);
+            peers &= r & b ? set : ~set;
+          }
         }
+        int pos = mine ? counters[wave][r] : 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if(mine) {
-          int pos = counters[wave][r];
           order[pos + popc(peers & lanemask_lt(lane))] = t + 64 * u + lane;
           // The last of the peers moves the counter on.
           if(!(peers & ~lanemask_le(lane)))
@@ -174,7 +184,8 @@ struct embedding_plan_f {
 
 template<typename grad_t, typename out_t>
 struct embedding_sum_f {
-  enum { W = row_chunk_t<grad_t>::width, batch = 4 };
+  enum { W = row_chunk_t<grad_t>::width, batch = 8,
+    group_rows = 8, min_cols = 8, max_groups = embedding_nt / min_cols };
   const grad_t* grad;
   int64_t grad_stride;
   int num_rows, dim;
@@ -187,27 +198,33 @@ struct embedding_sum_f {
   const int* order;
   float* partials;              // two rows of dim per block
   int cols, rows, col_blocks;   // threads along a row, groups of them, blocks
-  int rows_per_group, row_ctas;
+  int block_ctas;               // CTAs for blocks of long rows, the first ones
 
-  // sum += the tokens order[begin .. end) of the thread's columns.
-  MGPU_DEVICE void add(int begin, int end, int col, float (&sum)[W]) const {
+  // Every token of [begin, end) in sorted order, `batch` rows on their way at
+  // a time, the next ones' places fetched meanwhile: use(i, values).
+  template<typename use_t>
+  __forceinline__ MGPU_DEVICE void each(int begin, int end, int col, use_t use)
+    const {
+    int at[batch];
+    PRAGMA_UNROLL
+    for(int u = 0; u < batch; ++u) at[u] = begin + u < end ? order[begin + u] : 0;
+    PRAGMA_NO_UNROLL
     for(int i = begin; i < end; i += batch) {
-      row_chunk_t<grad_t> c[batch];
+      row_held_t<grad_t> c[batch];
       PRAGMA_UNROLL
       for(int u = 0; u < batch; ++u)
         if(i + u < end)
-          c[u].load(grad + order[i + u] * grad_stride + col, dim - col,
-            (grad_t)0.f);
+          c[u].load(grad + at[u] * grad_stride + col, dim - col, (grad_t)0.f);
       PRAGMA_UNROLL
       for(int u = 0; u < batch; ++u)
-        if(i + u < end) {
-          PRAGMA_UNROLL
-          for(int j = 0; j < W; ++j) sum[j] += (float)c[u].x[j];
-        }
+        at[u] = i + batch + u < end ? order[i + batch + u] : 0;
+      PRAGMA_UNROLL
+      for(int u = 0; u < batch; ++u) if(i + u < end) use(i + u, c[u]);
     }
   }
 
-  MGPU_DEVICE void write(int v, int col, const float (&sum)[W]) const {
+  __forceinline__ MGPU_DEVICE void write(int v, int col, const float (&sum)[W])
+    const {
     out_t* p = output + v * output_stride + col;
     row_values_t<out_t, W> x;
     if(accumulate) {
@@ -223,62 +240,92 @@ struct embedding_sum_f {
   }
 
   MGPU_DEVICE void operator()(int tid, int cta) const {
-    int block = cta / col_blocks;
+    __shared__ int shared_starts[max_groups][group_rows + 1];
     int group = tid / cols;
     int col = (cta % col_blocks * cols + tid % cols) * W;
-    if(col >= dim) return;
-    if(block < row_ctas) {
-      int v0 = (block * rows + group) * rows_per_group;
-      int v1 = min(v0 + rows_per_group, num_rows);
-      if(v0 >= num_rows) return;
-      int begin = starts[v0];
-      for(int v = v0; v < v1; ++v) {
-        int end = starts[v + 1], n = end - begin;
-        if(n <= embedding_block && (n || !accumulate)) {
-          float sum[W] = { };
-          add(begin, end, col, sum);
-          write(v, col, sum);
-        }
-        begin = end;
-      }
-    } else {
+    int block = cta / col_blocks;
+    float sum[W] = { };
+    auto add = [&](int, const row_held_t<grad_t>& c) {
+      PRAGMA_UNROLL
+      for(int j = 0; j < W; ++j) sum[j] += c.get(j);
+    };
+    if(block < block_ctas) {
       // Block b of the sorted tokens: what of it belongs to long rows, which
       // are the one of its first token and the one of its last.
-      int b = (block - row_ctas) * rows + group;
+      int b = block * rows + group;
       int total = starts[num_rows];
       int begin = b * embedding_block;
-      if(begin >= total) return;
+      if(begin >= total || col >= dim) return;
       int end = min(begin + (int)embedding_block, total);
       int first = ids[order[begin]], last = ids[order[end - 1]];
       int first_end = starts[first + 1];
       if(first_end - starts[first] > embedding_block) {
-        float sum[W] = { };
-        add(begin, min(first_end, end), col, sum);
+        each(begin, min(first_end, end), col, add);
         store_partial(2 * b, col, sum);
       }
       if(last != first) {
         int last_begin = starts[last];
         if(starts[last + 1] - last_begin > embedding_block) {
-          float sum[W] = { };
-          add(last_begin, end, col, sum);
+          PRAGMA_UNROLL
+          for(int j = 0; j < W; ++j) sum[j] = 0;
+          each(last_begin, end, col, add);
           store_partial(2 * b + 1, col, sum);
         }
       }
+      return;
+    }
+
+    int v0 = ((block - block_ctas) * rows + group) * group_rows;
+    for(int i = tid % cols; i <= group_rows; i += cols)
+      if(group < rows)
+        shared_starts[group][i] = starts[min(v0 + i, num_rows)];
+    __syncthreads();
+    if(v0 >= num_rows || col >= dim) return;
+    const int* at = shared_starts[group];
+    int r = 0, end = at[1];     // the row at hand, and where its tokens end
+    // Rows in front of token i are done.  A long row's tokens are not among
+    // those looked at, and neither is it written.
+    auto finish = [&](int i) {
+      while(r < group_rows && v0 + r < num_rows && end <= i) {
+        int n = end - at[r];
+        if(n <= embedding_block && (n || !accumulate)) write(v0 + r, col, sum);
+        PRAGMA_UNROLL
+        for(int j = 0; j < W; ++j) sum[j] = 0;
+        ++r;
+        if(r < group_rows) end = at[r + 1];
+      }
+    };
+    int begin = at[0];
+    for(int next = 0; next < group_rows; ++next) {
+      // Runs of rows between long ones.
+      bool is_long = at[next + 1] - at[next] > embedding_block;
+      if(!is_long && next < group_rows - 1) continue;
+      int stop = is_long ? at[next] : at[next + 1];
+      each(begin, stop, col, [&](int i, const row_held_t<grad_t>& c) {
+        finish(i);
+        add(i, c);
+      });
+      finish(at[next + 1]);
+      begin = at[next + 1];
     }
   }
 
-  MGPU_DEVICE void store_partial(int slot, int col, const float (&sum)[W])
-    const {
+  __forceinline__ MGPU_DEVICE void store_partial(int slot, int col,
+    const float (&sum)[W]) const {
     float* p = partials + slot * (int64_t)dim + col;
+    row_values_t<float, W> x;
     PRAGMA_UNROLL
-    for(int j = 0; j < W; ++j) if(col + j < dim) p[j] = sum[j];
+    for(int j = 0; j < W; ++j) x.x[j] = sum[j];
+    x.store(p, dim - col);
   }
 };
 
-// One CTA per block of tokens and 64 columns; the CTA of a long row's first
+// One CTA per block of tokens and 256 columns; the CTA of a long row's first
 // block boundary joins the row, the others have nothing to do.
 template<typename out_t>
 struct embedding_long_f {
+  enum { B = embedding_block, groups = embedding_nt / 64, width = 4,
+    cta_cols = 64 * width };
   int num_rows, dim;
   float scale;
   int accumulate;
@@ -291,28 +338,38 @@ struct embedding_long_f {
   int col_blocks;
 
   MGPU_DEVICE void operator()(int tid, int cta) const {
-    enum { B = embedding_block, groups = embedding_nt / 64 };
-    __shared__ float shared[groups][64];
+    __shared__ float shared[groups][cta_cols];
     int b = cta / col_blocks;
     if(b * B >= starts[num_rows]) return;
     int v = ids[order[b * B]];
     int begin = starts[v], end = starts[v + 1];
     if(end - begin <= B || div_up(begin, (int)B) != b) return;
-    int col = cta % col_blocks * 64 + (tid & 63);
+    int lane = tid & 63, group = tid / 64;
+    int col = cta % col_blocks * cta_cols + lane * width;
     int blocks = div_up(end, (int)B);
-    float sum = 0;
+    float sum[width] = { };
     if(col < dim)
-      for(int i = begin / B + tid / 64; i < blocks; i += groups)
-        sum += partials[(2 * i + (i * B < begin)) * (int64_t)dim + col];
-    shared[tid / 64][tid & 63] = sum;
+      for(int i = begin / B + group; i < blocks; i += groups) {
+        row_values_t<float, width> x;
+        x.load(partials + (2 * i + (i * B < begin)) * (int64_t)dim + col,
+          dim - col);
+        PRAGMA_UNROLL
+        for(int j = 0; j < width; ++j) sum[j] += x.x[j];
+      }
+    PRAGMA_UNROLL
+    for(int j = 0; j < width; ++j) shared[group][lane + 64 * j] = sum[j];
     __syncthreads();
-    if(tid < 64 && col < dim) {
+    if(group || col >= dim) return;
+    PRAGMA_UNROLL
+    for(int j = 0; j < width; ++j) {
       PRAGMA_UNROLL
-      for(int g = 1; g < groups; ++g) sum += shared[g][tid];
-      sum *= scale;
-      out_t* p = output + v * output_stride + col;
-      if(accumulate) sum += (float)*p;
-      *p = (out_t)sum;
+      for(int g = 1; g < groups; ++g) sum[j] += shared[g][lane + 64 * j];
+      out_t* p = output + v * output_stride + col + j;
+      if(col + j < dim) {
+        float x = scale * sum[j];
+        if(accumulate) x += (float)*p;
+        *p = (out_t)x;
+      }
     }
   }
 };
@@ -374,18 +431,19 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
 
   typedef embedding_sum_f<grad_t, out_t> sum_t;
   embedding_shape_t shape(dim, sum_t::W);
-  int rows_per_group = 8;
-  int row_ctas = div_up(num_rows, shape.rows * rows_per_group);
+  int row_ctas = div_up(num_rows, shape.rows * (int)sum_t::group_rows);
+  int block_ctas = div_up(ws.blocks, shape.rows);
   sum_t sum { grad, grad_stride, num_rows, dim, scale, accumulate, output,
     output_stride, ids, starts, order, partials, shape.cols, shape.rows,
-    shape.col_blocks, rows_per_group, row_ctas };
-  cta_launch<embedding_nt>(sum, (row_ctas + div_up(ws.blocks, shape.rows)) *
-    shape.col_blocks, context);
+    shape.col_blocks, block_ctas };
+  cta_launch<embedding_nt>(sum, (block_ctas + row_ctas) * shape.col_blocks,
+    context);
 
   if(ws.blocks) {
-    int col_blocks = div_up(dim, 64);
-    embedding_long_f<out_t> join { num_rows, dim, scale, accumulate, output,
-      output_stride, ids, starts, order, partials, col_blocks };
+    typedef embedding_long_f<out_t> long_t;
+    int col_blocks = div_up(dim, (int)long_t::cta_cols);
+    long_t join { num_rows, dim, scale, accumulate, output, output_stride, ids,
+      starts, order, partials, col_blocks };
     cta_launch<embedding_nt>(join, ws.blocks * col_blocks, context);
   }
 }
