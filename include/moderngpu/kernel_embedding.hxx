@@ -35,7 +35,8 @@ inline bool embedding_grid_ok(int n, int dim) {
   return (int64_t)n * div_up((int64_t)dim, (int64_t)64) < ((int64_t)1 << 30);
 }
 
-template<typename type_t>
+// A thread moves `unroll` chunks of as many tokens, all on their way at once.
+template<typename type_t, int unroll>
 struct embedding_lookup_f {
   const type_t* table;
   int num_rows, dim;
@@ -45,22 +46,33 @@ struct embedding_lookup_f {
   float scale;
   type_t* output;
   int64_t output_stride;
-  int cols, rows, col_blocks;
+  int cols, rows, col_blocks, stream;
 
   MGPU_DEVICE void operator()(int tid, int cta) const {
-    typedef row_chunk_t<type_t> chunk_t;
-    int t = cta / col_blocks * rows + tid / cols;
-    int col = (cta % col_blocks * cols + tid % cols) * chunk_t::width;
-    if(t >= count || col >= dim) return;
-    int id = ids[t];
-    bool inside = (unsigned)id < (unsigned)num_rows;
-    chunk_t c;
-    if(inside)
-      c.load(table + id * row_stride + col, dim - col, (type_t)0.f);
+    typedef row_held_t<type_t> held_t;
+    int t = cta / col_blocks * (rows * unroll) + tid / cols;
+    int col = (cta % col_blocks * cols + tid % cols) * held_t::width;
+    if(col >= dim) return;
+    int id[unroll];
     PRAGMA_UNROLL
-    for(int i = 0; i < chunk_t::width; ++i)
-      c.x[i] = (type_t)(inside ? scale * (float)c.x[i] : 0.f);
-    c.store(output + t * output_stride + col, dim - col);
+    for(int u = 0; u < unroll; ++u)
+      id[u] = t + u * rows < count ? ids[t + u * rows] : -1;
+    held_t c[unroll];
+    PRAGMA_UNROLL
+    for(int u = 0; u < unroll; ++u)
+      if((unsigned)id[u] < (unsigned)num_rows)
+        c[u].load(table + id[u] * row_stride + col, dim - col, (type_t)0.f);
+    PRAGMA_UNROLL
+    for(int u = 0; u < unroll; ++u) {
+      bool inside = (unsigned)id[u] < (unsigned)num_rows;
+      float x[held_t::width];
+      PRAGMA_UNROLL
+      for(int i = 0; i < held_t::width; ++i)
+        x[i] = inside ? scale * c[u].get(i) : 0.f;
+      if(t + u * rows < count)
+        row_store(x, output + (t + u * rows) * output_stride + col, dim - col,
+          stream);
+    }
   }
 };
 
@@ -75,7 +87,7 @@ struct embedding_lookup_f {
 // launch, so that no CTA adds more than rows-per-CTA * embedding_block rows.
 
 enum { embedding_plan_nt = 1024, embedding_plan_rows = 512,
-  embedding_block = 64 };
+  embedding_block = 32 };
 
 // Each CTA takes embedding_plan_rows consecutive rows and looks at every id:
 // those below its rows count towards where its tokens begin, those inside are
@@ -161,11 +173,24 @@ struct embedding_plan_f {
         lanemask_t peers = ballot(mine);
         if(!peers) continue;
         if(peers & (peers - 1)) {
-          // More than one: those with the same row.
+          // More than one: those with the same row.  Few rows (a frequent
+          // token) one after the other, many by the bits of their numbers.
+          lanemask_t inside = peers, rest = inside;
+          int tries = 0;
           PRAGMA_NO_UNROLL
-          for(int b = 1; b < R; b *= 2) {
-            lanemask_t set = ballot(r & b);
-            peers &= r & b ? set : ~set;
+          do {
+            int row = readlane(r, ffs(rest) - 1);
+            lanemask_t same = ballot(mine && r == row);
+            if(same >> lane & 1) peers = same;
+            rest &= ~same;
+          } while(rest && ++tries < 4);
+          if(rest) {
+            peers = inside;
+            PRAGMA_NO_UNROLL
+            for(int b = 1; b < R; b *= 2) {
+              lanemask_t set = ballot(r & b);
+              peers &= r & b ? set : ~set;
+            }
           }
         }
         int pos = mine ? counters[wave][r] : 0;
@@ -184,13 +209,19 @@ struct embedding_plan_f {
 
 template<typename grad_t, typename out_t>
 struct embedding_sum_f {
-  enum { W = row_chunk_t<grad_t>::width, batch = 8,
-    group_rows = 8, min_cols = 8, max_groups = embedding_nt / min_cols };
+  // As many values as make 16 bytes of the result: a wave's stores then fill
+  // whole lines.  (16-bit gradients into a 32-bit table with 8 values a thread
+  // leave gaps between a store's lanes; streamed, that took 375 us where 264
+  // was without, two steps into 32768 x 4096.)
+  enum { W = row_chunk_t<out_t>::width, batch = 8,
+    max_rows = 8, min_cols = 8, max_groups = embedding_nt / min_cols };
+  typedef row_held_t<grad_t, W> held_t;
+  typedef row_held_t<out_t> held_out_t;
   const grad_t* grad;
   int64_t grad_stride;
   int num_rows, dim;
   float scale;
-  int accumulate;
+  int accumulate, stream;
   out_t* output;
   int64_t output_stride;
   const int* ids;
@@ -198,6 +229,7 @@ struct embedding_sum_f {
   const int* order;
   float* partials;              // two rows of dim per block
   int cols, rows, col_blocks;   // threads along a row, groups of them, blocks
+  int group_rows;               // rows per group, at most max_rows
   int block_ctas;               // CTAs for blocks of long rows, the first ones
 
   // Every token of [begin, end) in sorted order, `batch` rows on their way at
@@ -210,7 +242,7 @@ struct embedding_sum_f {
     for(int u = 0; u < batch; ++u) at[u] = begin + u < end ? order[begin + u] : 0;
     PRAGMA_NO_UNROLL
     for(int i = begin; i < end; i += batch) {
-      row_held_t<grad_t> c[batch];
+      held_t c[batch];
       PRAGMA_UNROLL
       for(int u = 0; u < batch; ++u)
         if(i + u < end)
@@ -226,26 +258,25 @@ struct embedding_sum_f {
   __forceinline__ MGPU_DEVICE void write(int v, int col, const float (&sum)[W])
     const {
     out_t* p = output + v * output_stride + col;
-    row_values_t<out_t, W> x;
+    float x[W];
+    PRAGMA_UNROLL
+    for(int j = 0; j < W; ++j) x[j] = scale * sum[j];
     if(accumulate) {
-      x.load(p, dim - col);
+      held_out_t before;
+      before.load(p, dim - col, (out_t)0.f);
       PRAGMA_UNROLL
-      for(int j = 0; j < W; ++j)
-        x.x[j] = (out_t)((float)x.x[j] + scale * sum[j]);
-    } else {
-      PRAGMA_UNROLL
-      for(int j = 0; j < W; ++j) x.x[j] = (out_t)(scale * sum[j]);
+      for(int j = 0; j < W; ++j) x[j] += before.get(j);
     }
-    x.store(p, dim - col);
+    row_store(x, p, dim - col, stream);
   }
 
   MGPU_DEVICE void operator()(int tid, int cta) const {
-    __shared__ int shared_starts[max_groups][group_rows + 1];
+    __shared__ int shared_starts[max_groups][max_rows + 1];
     int group = tid / cols;
     int col = (cta % col_blocks * cols + tid % cols) * W;
     int block = cta / col_blocks;
     float sum[W] = { };
-    auto add = [&](int, const row_held_t<grad_t>& c) {
+    auto add = [&](int, const held_t& c) {
       PRAGMA_UNROLL
       for(int j = 0; j < W; ++j) sum[j] += c.get(j);
     };
@@ -301,7 +332,7 @@ struct embedding_sum_f {
       bool is_long = at[next + 1] - at[next] > embedding_block;
       if(!is_long && next < group_rows - 1) continue;
       int stop = is_long ? at[next] : at[next + 1];
-      each(begin, stop, col, [&](int i, const row_held_t<grad_t>& c) {
+      each(begin, stop, col, [&](int i, const held_t& c) {
         finish(i);
         add(i, c);
       });
@@ -324,7 +355,7 @@ struct embedding_sum_f {
 // block boundary joins the row, the others have nothing to do.
 template<typename out_t>
 struct embedding_long_f {
-  enum { B = embedding_block, groups = embedding_nt / 64, width = 4,
+  enum { B = embedding_block, groups = embedding_nt / 64, width = 4, batch = 8,
     cta_cols = 64 * width };
   int num_rows, dim;
   float scale;
@@ -349,12 +380,21 @@ struct embedding_long_f {
     int blocks = div_up(end, (int)B);
     float sum[width] = { };
     if(col < dim)
-      for(int i = begin / B + group; i < blocks; i += groups) {
-        row_values_t<float, width> x;
-        x.load(partials + (2 * i + (i * B < begin)) * (int64_t)dim + col,
-          dim - col);
+      for(int i = begin / B + group; i < blocks; i += batch * groups) {
+        row_held_t<float> x[batch];
         PRAGMA_UNROLL
-        for(int j = 0; j < width; ++j) sum[j] += x.x[j];
+        for(int u = 0; u < batch; ++u) {
+          int at = i + u * groups;
+          if(at < blocks)
+            x[u].load(partials + (2 * at + (at * B < begin)) * (int64_t)dim +
+              col, dim - col, 0.f);
+        }
+        PRAGMA_UNROLL
+        for(int u = 0; u < batch; ++u) {
+          PRAGMA_UNROLL
+          for(int j = 0; j < width; ++j)
+            if(i + u * groups < blocks) sum[j] += x[u].get(j);
+        }
       }
     PRAGMA_UNROLL
     for(int j = 0; j < width; ++j) shared[group][lane + 64 * j] = sum[j];
@@ -385,11 +425,21 @@ void embedding_lookup(const type_t* table, int num_rows, int dim,
   int64_t output_stride, context_t& context) {
   if(count <= 0 || dim <= 0) return;
   detail::embedding_shape_t shape(dim, detail::row_chunk_t<type_t>::width);
-  detail::embedding_lookup_f<type_t> k { table, num_rows, dim, row_stride,
-    ids, count, scale, output, output_stride, shape.cols, shape.rows,
-    shape.col_blocks };
-  cta_launch<detail::embedding_nt>(k,
-    div_up(count, shape.rows) * shape.col_blocks, context);
+  int stream = (int64_t)count * dim * (int64_t)sizeof(type_t) >=
+    detail::row_stream_bytes;
+  auto launch = [&](auto unroll) {
+    detail::embedding_lookup_f<type_t, decltype(unroll)::value> k { table,
+      num_rows, dim, row_stride, ids, count, scale, output, output_stride,
+      shape.cols, shape.rows, shape.col_blocks, stream };
+    cta_launch<detail::embedding_nt>(k, div_up(count, shape.rows *
+      decltype(unroll)::value) * shape.col_blocks, context);
+  };
+  // Four tokens a thread once that leaves 2048 CTAs, all that fit the device
+  // at once.
+  if((int64_t)div_up(count, 4 * shape.rows) * shape.col_blocks >= 2048)
+    launch(std::integral_constant<int, 4>());
+  else
+    launch(std::integral_constant<int, 1>());
 }
 
 namespace detail {
@@ -431,11 +481,17 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
 
   typedef embedding_sum_f<grad_t, out_t> sum_t;
   embedding_shape_t shape(dim, sum_t::W);
-  int row_ctas = div_up(num_rows, shape.rows * (int)sum_t::group_rows);
+  // A group's tokens come one batch after the other: about 16 of them, and as
+  // many rows as have that many on average.
+  int group_rows = (int)max((int64_t)1, min((int64_t)sum_t::max_rows,
+    (int64_t)16 * num_rows / max(count, 1)));
+  int row_ctas = div_up(num_rows, shape.rows * group_rows);
   int block_ctas = div_up(ws.blocks, shape.rows);
-  sum_t sum { grad, grad_stride, num_rows, dim, scale, accumulate, output,
+  int stream = !accumulate &&
+    (int64_t)num_rows * dim * (int64_t)sizeof(out_t) >= row_stream_bytes;
+  sum_t sum { grad, grad_stride, num_rows, dim, scale, accumulate, stream, output,
     output_stride, ids, starts, order, partials, shape.cols, shape.rows,
-    shape.col_blocks, block_ctas };
+    shape.col_blocks, group_rows, block_ctas };
   cta_launch<embedding_nt>(sum, (block_ctas + row_ctas) * shape.col_blocks,
     context);
 

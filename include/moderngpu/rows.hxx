@@ -31,6 +31,22 @@ template<> struct __attribute__((packed, aligned(4))) row_words_at_t<4> {
   row_words_t w;
 };
 
+// 16 bytes past the caches' replacement order, to any multiple of 2 or 4: for
+// results that are larger than the caches, so that they do not displace what
+// is read again.  Only whole lines gain: the lanes of a wave have to write one
+// after the other.
+typedef row_words_t row_words_any2_t __attribute__((aligned(2)));
+typedef row_words_t row_words_any4_t __attribute__((aligned(4)));
+template<int alignment>
+MGPU_DEVICE inline void row_stream(row_words_t w, void* p) {
+  if constexpr(2 == alignment)
+    __builtin_nontemporal_store(w, (row_words_any2_t*)p);
+  else
+    __builtin_nontemporal_store(w, (row_words_any4_t*)p);
+}
+// Results of at least this many bytes are streamed.
+enum : int64_t { row_stream_bytes = 64 << 20 };
+
 template<typename type_t>
 struct row_chunk_t {
   enum { width = 16 / sizeof(type_t) };
@@ -50,13 +66,14 @@ struct row_chunk_t {
       for(int i = 0; i < width; ++i) x[i] = i < n ? p[i] : rest;
     }
   }
-  MGPU_DEVICE void store_all(type_t* p) const {
+  MGPU_DEVICE void store_all(type_t* p, bool stream) const {
     row_words_t w;
     __builtin_memcpy(&w, x, 16);
-    ((any_words_t*)p)->w = w;
+    if(stream) row_stream<sizeof(type_t)>(w, p);
+    else ((any_words_t*)p)->w = w;
   }
-  MGPU_DEVICE void store(type_t* p, int n) const {
-    if(n >= width) store_all(p);
+  MGPU_DEVICE void store(type_t* p, int n, bool stream = false) const {
+    if(n >= width) store_all(p, stream);
     else {
       PRAGMA_UNROLL
       for(int i = 0; i < width; ++i) if(i < n) p[i] = x[i];
@@ -66,21 +83,25 @@ struct row_chunk_t {
 
 // A chunk that stays as its four words and is taken apart where it is used:
 // 16-bit values that live long as separate ones would take twice the registers.
-template<typename type_t>
+template<typename type_t, int width_ = 16 / sizeof(type_t)>
 struct row_held_t {
-  enum { width = 16 / sizeof(type_t) };
-  typedef row_words_at_t<sizeof(type_t)> any_words_t;
-  unsigned w[4];
+  enum { width = width_, words = width * sizeof(type_t) / 4 };
+  typedef unsigned words_t __attribute__((ext_vector_type(words)));
+  struct __attribute__((packed, aligned(sizeof(type_t)))) any_words_t {
+    words_t w;
+  };
+  unsigned w[words];
 
   __forceinline__ MGPU_DEVICE void load(const type_t* p, int n, type_t rest) {
-    row_words_t x;
-    if(n >= width) x = ((const any_words_t*)p)->w;
-    else {
-      row_chunk_t<type_t> ch;
-      ch.load(p, n, rest);
-      __builtin_memcpy(&x, ch.x, 16);
+    if(n >= width) {
+      words_t x = ((const any_words_t*)p)->w;
+      __builtin_memcpy(w, &x, sizeof(w));
+    } else {
+      type_t x[width];
+      PRAGMA_UNROLL
+      for(int i = 0; i < width; ++i) x[i] = i < n ? p[i] : rest;
+      __builtin_memcpy(w, x, sizeof(w));
     }
-    __builtin_memcpy(w, &x, 16);
   }
   __forceinline__ MGPU_DEVICE float get(int i) const {
     if constexpr(std::is_same<type_t, bf16_t>::value)
@@ -96,7 +117,8 @@ struct row_held_t {
   // kept for later.
   __forceinline__ MGPU_DEVICE void renew() {
 #ifdef __HIP_DEVICE_COMPILE__
-    asm("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
+    PRAGMA_UNROLL
+    for(int i = 0; i < words; ++i) asm("" : "+v"(w[i]));
 #endif
   }
 };
@@ -104,7 +126,8 @@ struct row_held_t {
 // width floats, each rounded to the row's type, to n of its values at p.
 template<typename type_t>
 __forceinline__ MGPU_DEVICE void row_store(
-  const float (&x)[row_chunk_t<type_t>::width], type_t* p, int n) {
+  const float (&x)[row_chunk_t<type_t>::width], type_t* p, int n,
+  bool stream = false) {
   typedef float pair_t __attribute__((ext_vector_type(2)));
   typedef type_t two_t __attribute__((ext_vector_type(2)));
   row_chunk_t<type_t> ch;
@@ -115,7 +138,7 @@ __forceinline__ MGPU_DEVICE void row_store(
     ch.x[i] = t.x;
     ch.x[i + 1] = t.y;
   }
-  ch.store(p, n);
+  ch.store(p, n, stream);
 }
 
 // `width` values of a row, in 16-byte moves where they fill some: the results
@@ -135,13 +158,13 @@ struct row_values_t {
       for(int j = 0; j < W; ++j) x[i + j] = c.x[j];
     }
   }
-  MGPU_DEVICE void store(type_t* p, int n) const {
+  MGPU_DEVICE void store(type_t* p, int n, bool stream = false) const {
     PRAGMA_UNROLL
     for(int i = 0; i < width; i += W) {
       row_chunk_t<type_t> c;
       PRAGMA_UNROLL
       for(int j = 0; j < W; ++j) c.x[j] = x[i + j];
-      c.store(p + i, n - i);
+      c.store(p + i, n - i, stream);
     }
   }
 };
