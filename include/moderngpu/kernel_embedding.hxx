@@ -36,7 +36,7 @@ inline bool embedding_grid_ok(int n, int dim) {
 }
 
 // A thread moves `unroll` chunks of as many tokens, all on their way at once.
-template<typename type_t, int unroll>
+template<typename type_t, int unroll, bool stream>
 struct embedding_lookup_f {
   const type_t* table;
   int num_rows, dim;
@@ -46,7 +46,7 @@ struct embedding_lookup_f {
   float scale;
   type_t* output;
   int64_t output_stride;
-  int cols, rows, col_blocks, stream;
+  int cols, rows, col_blocks;
 
   MGPU_DEVICE void operator()(int tid, int cta) const {
     typedef row_held_t<type_t> held_t;
@@ -70,8 +70,8 @@ struct embedding_lookup_f {
       for(int i = 0; i < held_t::width; ++i)
         x[i] = inside ? scale * c[u].get(i) : 0.f;
       if(t + u * rows < count)
-        row_store(x, output + (t + u * rows) * output_stride + col, dim - col,
-          stream);
+        row_store<stream>(x, output + (t + u * rows) * output_stride + col,
+          dim - col);
     }
   }
 };
@@ -207,7 +207,7 @@ struct embedding_plan_f {
   }
 };
 
-template<typename grad_t, typename out_t>
+template<typename grad_t, typename out_t, bool stream>
 struct embedding_sum_f {
   // As many values as make 16 bytes of the result: a wave's stores then fill
   // whole lines.  (16-bit gradients into a 32-bit table with 8 values a thread
@@ -221,7 +221,7 @@ struct embedding_sum_f {
   int64_t grad_stride;
   int num_rows, dim;
   float scale;
-  int accumulate, stream;
+  int accumulate;
   out_t* output;
   int64_t output_stride;
   const int* ids;
@@ -267,7 +267,7 @@ struct embedding_sum_f {
       PRAGMA_UNROLL
       for(int j = 0; j < W; ++j) x[j] += before.get(j);
     }
-    row_store(x, p, dim - col, stream);
+    row_store<stream>(x, p, dim - col);
   }
 
   MGPU_DEVICE void operator()(int tid, int cta) const {
@@ -425,21 +425,24 @@ void embedding_lookup(const type_t* table, int num_rows, int dim,
   int64_t output_stride, context_t& context) {
   if(count <= 0 || dim <= 0) return;
   detail::embedding_shape_t shape(dim, detail::row_chunk_t<type_t>::width);
-  int stream = (int64_t)count * dim * (int64_t)sizeof(type_t) >=
-    detail::row_stream_bytes;
-  auto launch = [&](auto unroll) {
-    detail::embedding_lookup_f<type_t, decltype(unroll)::value> k { table,
-      num_rows, dim, row_stride, ids, count, scale, output, output_stride,
-      shape.cols, shape.rows, shape.col_blocks, stream };
+  auto launch = [&](auto unroll, auto stream) {
+    enum { tokens = decltype(unroll)::value };
+    detail::embedding_lookup_f<type_t, tokens, decltype(stream)::value> k {
+      table, num_rows, dim, row_stride, ids, count, scale, output,
+      output_stride, shape.cols, shape.rows, shape.col_blocks };
     cta_launch<detail::embedding_nt>(k, div_up(count, shape.rows *
-      decltype(unroll)::value) * shape.col_blocks, context);
+      (int)tokens) * shape.col_blocks, context);
   };
   // Four tokens a thread once that leaves 2048 CTAs, all that fit the device
   // at once.
-  if((int64_t)div_up(count, 4 * shape.rows) * shape.col_blocks >= 2048)
-    launch(std::integral_constant<int, 4>());
+  bool many = (int64_t)div_up(count, 4 * shape.rows) * shape.col_blocks >= 2048;
+  if((int64_t)count * dim * (int64_t)sizeof(type_t) >=
+    detail::row_stream_bytes)
+    launch(std::integral_constant<int, 4>(), std::true_type());
+  else if(many)
+    launch(std::integral_constant<int, 4>(), std::false_type());
   else
-    launch(std::integral_constant<int, 1>());
+    launch(std::integral_constant<int, 1>(), std::false_type());
 }
 
 namespace detail {
@@ -479,21 +482,27 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
   cta_launch<embedding_plan_nt>(plan, div_up(num_rows,
     (int)embedding_plan_rows), context);
 
-  typedef embedding_sum_f<grad_t, out_t> sum_t;
-  embedding_shape_t shape(dim, sum_t::W);
-  // A group's tokens come one batch after the other: about 16 of them, and as
-  // many rows as have that many on average.
-  int group_rows = (int)max((int64_t)1, min((int64_t)sum_t::max_rows,
-    (int64_t)16 * num_rows / max(count, 1)));
-  int row_ctas = div_up(num_rows, shape.rows * group_rows);
-  int block_ctas = div_up(ws.blocks, shape.rows);
-  int stream = !accumulate &&
-    (int64_t)num_rows * dim * (int64_t)sizeof(out_t) >= row_stream_bytes;
-  sum_t sum { grad, grad_stride, num_rows, dim, scale, accumulate, stream, output,
-    output_stride, ids, starts, order, partials, shape.cols, shape.rows,
-    shape.col_blocks, group_rows, block_ctas };
-  cta_launch<embedding_nt>(sum, (block_ctas + row_ctas) * shape.col_blocks,
-    context);
+  auto add_up = [&](auto stream) {
+    typedef embedding_sum_f<grad_t, out_t, decltype(stream)::value> sum_t;
+    embedding_shape_t shape(dim, sum_t::W);
+    // A group's tokens come one batch after the other: about 16 of them, and
+    // as many rows as have that many on average.
+    int group_rows = (int)max((int64_t)1, min((int64_t)sum_t::max_rows,
+      (int64_t)16 * num_rows / max(count, 1)));
+    int row_ctas = div_up(num_rows, shape.rows * group_rows);
+    int block_ctas = div_up(ws.blocks, shape.rows);
+    sum_t sum { grad, grad_stride, num_rows, dim, scale, accumulate, output,
+      output_stride, ids, starts, order, partials, shape.cols, shape.rows,
+      shape.col_blocks, group_rows, block_ctas };
+    cta_launch<embedding_nt>(sum, (block_ctas + row_ctas) * shape.col_blocks,
+      context);
+  };
+  // (What is added to is read as well, and stays in the caches.)
+  if(!accumulate &&
+    (int64_t)num_rows * dim * (int64_t)sizeof(out_t) >= row_stream_bytes)
+    add_up(std::true_type());
+  else
+    add_up(std::false_type());
 
   if(ws.blocks) {
     typedef embedding_long_f<out_t> long_t;

@@ -34,7 +34,8 @@ template<> struct __attribute__((packed, aligned(4))) row_words_at_t<4> {
 // 16 bytes past the caches' replacement order, to any multiple of 2 or 4: for
 // results that are larger than the caches, so that they do not displace what
 // is read again.  Only whole lines gain: the lanes of a wave have to write one
-// after the other.
+// after the other.  (A choice of the two stores at run time does not survive
+// the compiler, which joins them into the plain one.)
 typedef row_words_t row_words_any2_t __attribute__((aligned(2)));
 typedef row_words_t row_words_any4_t __attribute__((aligned(4)));
 template<int alignment>
@@ -66,14 +67,14 @@ struct row_chunk_t {
       for(int i = 0; i < width; ++i) x[i] = i < n ? p[i] : rest;
     }
   }
-  MGPU_DEVICE void store_all(type_t* p, bool stream) const {
-    row_words_t w;
-    __builtin_memcpy(&w, x, 16);
-    if(stream) row_stream<sizeof(type_t)>(w, p);
-    else ((any_words_t*)p)->w = w;
-  }
-  MGPU_DEVICE void store(type_t* p, int n, bool stream = false) const {
-    if(n >= width) store_all(p, stream);
+  template<bool stream = false>
+  MGPU_DEVICE void store(type_t* p, int n) const {
+    if(n >= width) {
+      row_words_t w;
+      __builtin_memcpy(&w, x, 16);
+      if constexpr(stream) row_stream<sizeof(type_t)>(w, p);
+      else ((any_words_t*)p)->w = w;
+    }
     else {
       PRAGMA_UNROLL
       for(int i = 0; i < width; ++i) if(i < n) p[i] = x[i];
@@ -124,10 +125,9 @@ struct row_held_t {
 };
 
 // width floats, each rounded to the row's type, to n of its values at p.
-template<typename type_t>
+template<bool stream = false, typename type_t>
 __forceinline__ MGPU_DEVICE void row_store(
-  const float (&x)[row_chunk_t<type_t>::width], type_t* p, int n,
-  bool stream = false) {
+  const float (&x)[row_chunk_t<type_t>::width], type_t* p, int n) {
   typedef float pair_t __attribute__((ext_vector_type(2)));
   typedef type_t two_t __attribute__((ext_vector_type(2)));
   row_chunk_t<type_t> ch;
@@ -138,7 +138,7 @@ __forceinline__ MGPU_DEVICE void row_store(
     ch.x[i] = t.x;
     ch.x[i + 1] = t.y;
   }
-  ch.store(p, n, stream);
+  ch.template store<stream>(p, n);
 }
 
 // `width` values of a row, in 16-byte moves where they fill some: the results
@@ -158,13 +158,13 @@ struct row_values_t {
       for(int j = 0; j < W; ++j) x[i + j] = c.x[j];
     }
   }
-  MGPU_DEVICE void store(type_t* p, int n, bool stream = false) const {
+  MGPU_DEVICE void store(type_t* p, int n) const {
     PRAGMA_UNROLL
     for(int i = 0; i < width; i += W) {
       row_chunk_t<type_t> c;
       PRAGMA_UNROLL
       for(int j = 0; j < W; ++j) c.x[j] = x[i + j];
-      c.store(p + i, n - i, stream);
+      c.store(p + i, n - i);
     }
   }
 };
