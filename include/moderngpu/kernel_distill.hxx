@@ -30,6 +30,9 @@ enum distill_mode_t { distill_loss_only, distill_grad_only, distill_both };
 // registers between the pass that sums it and the pass that writes the
 // gradient, and is read once; its loads are all in flight while the teacher's
 // entries are dealt with.  What a longer row has behind that is read by both.
+// The gradient is streamed past the caches, which the rows being read need (4096
+// x 32768 bf16: 94 us against 112, 2048 x 65536: 101 against 113; 64 rows of
+// 131072 take 24 either way).
 template<typename type_t, typename teacher_t, distill_mode_t mode, int nt_,
   int chunks>
 struct distill_f {
@@ -101,7 +104,7 @@ struct distill_f {
     float x[W];
     PRAGMA_UNROLL
     for(int i = 0; i < W; ++i) x[i] = scale * share(ch.get(i), m);
-    row_store(x, dz + v, vocab - v);
+    row_store<true>(x, dz + v, vocab - v);
   }
 
   // What of the row is not held, four chunks of the thread at a time.
@@ -324,7 +327,7 @@ void distill_launch(const type_t* logits, int64_t stride, int rows, int vocab,
     // on a CU.  Past 32768 16-bit values that is one row in all its registers,
     // and two rows of which each holds half are faster (2048 x 65536 bf16: 114
     // us against 191 with 1024 threads, x 131072: 242 against 280; two that
-    // hold a quarter: 121 and 272).  32-bit rows have half the arithmetic a
+    // hold a quarter: 121 and 272; all before the stores were streamed).  32-bit rows have half the arithmetic a
     // byte, and one row held by 1024 threads does (1024 x 65536: 128 us
     // against 133, x 131072: 254 against 289).
     if(vocab <= 256 * 4 * W)
