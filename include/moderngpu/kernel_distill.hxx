@@ -30,9 +30,9 @@ enum distill_mode_t { distill_loss_only, distill_grad_only, distill_both };
 // registers between the pass that sums it and the pass that writes the
 // gradient, and is read once; its loads are all in flight while the teacher's
 // entries are dealt with.  What a longer row has behind that is read by both.
-// The gradient is streamed past the caches, which the rows being read need (4096
-// x 32768 bf16: 94 us against 112, 2048 x 65536: 101 against 113; 64 rows of
-// 131072 take 24 either way).
+// The gradient is streamed past the caches, which the rows being read need (2048
+// x 131072 bf16: 222 us against 243, 333 x 50021 fp32 in two calls: 40.5 against
+// 43.6; 4096 x 32768 bf16 with a fifth of the rows masked: 102 against 100).
 template<typename type_t, typename teacher_t, distill_mode_t mode, int nt_,
   int chunks>
 struct distill_f {
@@ -194,7 +194,7 @@ struct distill_f {
         PRAGMA_UNROLL
         for(int i = 0; i < W; ++i) zero.x[i] = (type_t)0.f;
         for(int v = tid * W; v < vocab; v += nt * W)
-          zero.store(dz + v, vocab - v);
+          zero.template store<true>(dz + v, vocab - v);
       }
       return;
     }
