@@ -351,7 +351,11 @@ MGPU_HIP_API int mgpu_hip_inner_join_pairs(int a_count, int b_count,
  *    row to the next.  Inputs take any stride >= 0 (0: the same row again);
  *    an output's is at least its row length.  Pointers are aligned to one
  *    value, nothing more.
- *  - An output may not overlap an input, except where it says so. */
+ *  - An output may not overlap an input, except where it says so; a matrix
+ *    takes everything from its first value to its last, gaps between its rows
+ *    too.
+ *  - Numbers of tokens, rows of a table and values of a row go up to 2^30;
+ *    more is refused. */
 
 /* output[t] = scale * table[ids[t]] for t in [0, count): rows of dim values.
  * An id outside [0, num_rows) is padding and gives zeros. */

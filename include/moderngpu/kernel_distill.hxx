@@ -20,7 +20,7 @@
 
 BEGIN_MGPU_NAMESPACE
 
-enum { distill_max_top = 1024 };
+enum { distill_max_top = 1024, distill_max_vocab = 1 << 30 };
 
 namespace detail {
 
@@ -316,10 +316,16 @@ void distill_launch(const type_t* logits, int64_t stride, int rows, int vocab,
   if(rows <= 0) return;
   auto launch = [&](auto k) {
     typedef decltype(k) f_t;
-    f_t f { logits, stride, vocab, ids, teacher, top, tau,
-      (float)(1.4426950408889634 / tau), weights, loss, norms, grad,
-      grad_stride };
-    cta_launch<f_t::nt>(f, rows, context);
+    // (A launch counts its threads in 32 bits.)
+    const int most = 1 << 20;
+    for(int row = 0; row < rows; row += most) {
+      f_t f { logits + row * stride, stride, vocab,
+        ids + row * (int64_t)top, teacher + row * (int64_t)top, top, tau,
+        (float)(1.4426950408889634 / tau), weights ? weights + row : nullptr,
+        loss ? loss + row : nullptr, norms ? norms + 2 * (int64_t)row : nullptr,
+        grad ? grad + row * grad_stride : nullptr, grad_stride };
+      cta_launch<f_t::nt>(f, min(rows - row, most), context);
+    }
   };
   enum { W = row_chunk_t<type_t>::width };
   if constexpr(mode == distill_both) {

@@ -29,11 +29,12 @@ struct embedding_shape_t {
   }
 };
 
-// Whether the CTAs of the kernels below can be counted: no more than one a
-// token or row and 64 columns.
-inline bool embedding_grid_ok(int n, int dim) {
-  return (int64_t)n * div_up((int64_t)dim, (int64_t)64) < ((int64_t)1 << 30);
-}
+// Counts that the kernels below can index with.
+inline bool embedding_count_ok(int n) { return n <= 1 << 30; }
+
+// CTAs of one launch; more than that go in several (a launch counts its
+// threads in 32 bits).
+enum { embedding_grid = 1 << 18 };
 
 // A thread moves `unroll` chunks of as many tokens, all on their way at once.
 template<typename type_t, int unroll, bool stream>
@@ -121,7 +122,7 @@ struct embedding_plan_f {
     int v0 = cta * R;
     int rows = min((int)R, num_rows - v0);
 
-    // The wave's tokens (count < 2^30, see embedding_grid_ok).
+    // The wave's tokens (count <= 2^30, see embedding_count_ok).
     int piece = div_up(div_up(count, (int)W), 64) * 64;
     int begin = (int)min(wave * (int64_t)piece, (int64_t)count);
     int end = (int)min(begin + (int64_t)piece, (int64_t)count);
@@ -231,6 +232,7 @@ struct embedding_sum_f {
   int cols, rows, col_blocks;   // threads along a row, groups of them, blocks
   int group_rows;               // rows per group, at most max_rows
   int block_ctas;               // CTAs for blocks of long rows, the first ones
+  int first_block;              // (of this launch)
 
   // Every token of [begin, end) in sorted order, `batch` rows on their way at
   // a time, the next ones' places fetched meanwhile: use(i, values).
@@ -274,7 +276,7 @@ struct embedding_sum_f {
     __shared__ int shared_starts[max_groups][max_rows + 1];
     int group = tid / cols;
     int col = (cta % col_blocks * cols + tid % cols) * W;
-    int block = cta / col_blocks;
+    int block = first_block + cta / col_blocks;
     float sum[W] = { };
     auto add = [&](int, const held_t& c) {
       PRAGMA_UNROLL
@@ -306,6 +308,7 @@ struct embedding_sum_f {
       return;
     }
 
+    // (Rows of the last CTA may lie past the end, by less than 2^17.)
     int v0 = ((block - block_ctas) * rows + group) * group_rows;
     for(int i = tid % cols; i <= group_rows; i += cols)
       if(group < rows)
@@ -366,11 +369,11 @@ struct embedding_long_f {
   const int* starts;
   const int* order;
   const float* partials;
-  int col_blocks;
+  int col_blocks, first_block;
 
   MGPU_DEVICE void operator()(int tid, int cta) const {
     __shared__ float shared[groups][cta_cols];
-    int b = cta / col_blocks;
+    int b = first_block + cta / col_blocks;
     if(b * B >= starts[num_rows]) return;
     int v = ids[order[b * B]];
     int begin = starts[v], end = starts[v + 1];
@@ -427,11 +430,17 @@ void embedding_lookup(const type_t* table, int num_rows, int dim,
   detail::embedding_shape_t shape(dim, detail::row_chunk_t<type_t>::width);
   auto launch = [&](auto unroll, auto stream) {
     enum { tokens = decltype(unroll)::value };
-    detail::embedding_lookup_f<type_t, tokens, decltype(stream)::value> k {
-      table, num_rows, dim, row_stride, ids, count, scale, output,
-      output_stride, shape.cols, shape.rows, shape.col_blocks };
-    cta_launch<detail::embedding_nt>(k, div_up(count, shape.rows *
-      (int)tokens) * shape.col_blocks, context);
+    int per_cta = shape.rows * tokens;
+    int most = max(detail::embedding_grid / shape.col_blocks, 1) * per_cta;
+    for(int first = 0; first < count; first += most) {
+      int n = min(count - first, most);
+      detail::embedding_lookup_f<type_t, tokens, decltype(stream)::value> k {
+        table, num_rows, dim, row_stride, ids + first, n, scale,
+        output + first * output_stride, output_stride, shape.cols, shape.rows,
+        shape.col_blocks };
+      cta_launch<detail::embedding_nt>(k, div_up(n, per_cta) *
+        shape.col_blocks, context);
+    }
   };
   // Four tokens a thread once that leaves 2048 CTAs, all that fit the device
   // at once.
@@ -491,11 +500,14 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
       (int64_t)16 * num_rows / max(count, 1)));
     int row_ctas = div_up(num_rows, shape.rows * group_rows);
     int block_ctas = div_up(ws.blocks, shape.rows);
-    sum_t sum { grad, grad_stride, num_rows, dim, scale, accumulate, output,
-      output_stride, ids, starts, order, partials, shape.cols, shape.rows,
-      shape.col_blocks, group_rows, block_ctas };
-    cta_launch<embedding_nt>(sum, (block_ctas + row_ctas) * shape.col_blocks,
-      context);
+    int most = max(embedding_grid / shape.col_blocks, 1);
+    for(int first = 0; first < block_ctas + row_ctas; first += most) {
+      sum_t sum { grad, grad_stride, num_rows, dim, scale, accumulate, output,
+        output_stride, ids, starts, order, partials, shape.cols, shape.rows,
+        shape.col_blocks, group_rows, block_ctas, first };
+      cta_launch<embedding_nt>(sum, min(block_ctas + row_ctas - first, most) *
+        shape.col_blocks, context);
+    }
   };
   // (What is added to is read as well, and stays in the caches.)
   if(!accumulate &&
@@ -507,9 +519,13 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
   if(ws.blocks) {
     typedef embedding_long_f<out_t> long_t;
     int col_blocks = div_up(dim, (int)long_t::cta_cols);
-    long_t join { num_rows, dim, scale, accumulate, output, output_stride, ids,
-      starts, order, partials, col_blocks };
-    cta_launch<embedding_nt>(join, ws.blocks * col_blocks, context);
+    int most = max(embedding_grid / col_blocks, 1);
+    for(int first = 0; first < ws.blocks; first += most) {
+      long_t join { num_rows, dim, scale, accumulate, output, output_stride,
+        ids, starts, order, partials, col_blocks, first };
+      cta_launch<embedding_nt>(join, min(ws.blocks - first, most) * col_blocks,
+        context);
+    }
   }
 }
 

@@ -115,6 +115,13 @@ struct sample_settings_t {
   int top_k_all;
   float top_p_all, min_p_all;
 
+  // The rows from the n-th on.
+  void advance(int n) {
+    if(temperature) temperature += n;
+    if(top_k) top_k += n;
+    if(top_p) top_p += n;
+    if(min_p) min_p += n;
+  }
   __forceinline__ MGPU_DEVICE sample_row_t row(int r, int vocab) const {
     sample_row_t s;
     float t = temperature ? temperature[r] : temperature_all;
@@ -1337,38 +1344,48 @@ struct sample_row_f {
 
 inline int sample_pieces(int vocab) { return div_up(vocab, (int)sample_piece); }
 
-// Whether the CTAs can be counted.
-inline bool sample_grid_ok(int rows, int vocab) {
-  return (int64_t)rows * sample_pieces(vocab) < ((int64_t)1 << 31);
+// Rows that go together: their pieces' notes fit 80 MB and one launch.  More
+// rows take several rounds of launches with the same workspace.
+inline int sample_rows(int rows, int vocab) {
+  return min(rows, max(16384 / sample_pieces(vocab), 1));
 }
 
 inline size_t sample_workspace_bytes(int rows, int vocab) {
-  return sizeof(sample_piece_t) * (size_t)rows * sample_pieces(vocab);
+  return sizeof(sample_piece_t) * (size_t)sample_rows(rows, vocab) *
+    sample_pieces(vocab);
 }
 
 // workspace is 8-byte aligned.
 template<typename type_t>
 void sample_launch(const type_t* logits, int64_t stride, int rows, int vocab,
-  const float* uniform, const sample_settings_t& settings, int* token,
+  const float* uniform, sample_settings_t settings, int* token,
   float* logprob, void* workspace, context_t& context) {
-  if(rows <= 0) return;
   int bits = 0;
   while((1 << bits) < vocab) ++bits;
-  int pieces = sample_pieces(vocab);
-  sample_piece_t* from = (sample_piece_t*)workspace;
-  sample_piece_f<type_t> look { logits, stride, vocab, pieces, settings, from };
-  cta_launch<sample_piece_nt>(look, rows * pieces, context);
+  int pieces = sample_pieces(vocab), most = sample_rows(rows, vocab);
   sample_scale_t scale { min(62 - bits, 50) };
-  sample_weigh_f<type_t> weigh { logits, stride, vocab, pieces, scale, settings,
-    from };
+  sample_piece_t* from = (sample_piece_t*)workspace;
   // Not where all rows are known to have top-k, or neither top-p nor min-p.
-  if((settings.top_k || settings.top_k_all <= 0 || settings.top_k_all >= vocab) &&
-    (settings.top_p || settings.top_p_all < 1 || settings.min_p ||
-      settings.min_p_all > 0))
-    cta_launch<sample_piece_nt>(weigh, rows * pieces, context);
-  sample_row_f<type_t> draw { logits, stride, vocab, pieces, scale, uniform,
-    settings, from, token, logprob };
-  cta_launch<sample_nt>(draw, rows, context);
+  bool weighed = (settings.top_k || settings.top_k_all <= 0 ||
+    settings.top_k_all >= vocab) && (settings.top_p || settings.top_p_all < 1 ||
+    settings.min_p || settings.min_p_all > 0);
+  for(int row = 0; row < rows; row += most) {
+    int n = min(rows - row, most);
+    sample_piece_f<type_t> look { logits, stride, vocab, pieces, settings,
+      from };
+    cta_launch<sample_piece_nt>(look, n * pieces, context);
+    sample_weigh_f<type_t> weigh { logits, stride, vocab, pieces, scale,
+      settings, from };
+    if(weighed) cta_launch<sample_piece_nt>(weigh, n * pieces, context);
+    sample_row_f<type_t> draw { logits, stride, vocab, pieces, scale, uniform,
+      settings, from, token, logprob };
+    cta_launch<sample_nt>(draw, n, context);
+    logits += n * stride;
+    uniform += n;
+    token += n;
+    logprob += n;
+    settings.advance(n);
+  }
 }
 
 } // namespace detail

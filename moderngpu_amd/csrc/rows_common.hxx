@@ -54,7 +54,4 @@ struct matrix_t {
   }
 };
 
-// A grid that the launch front end can count.
-inline bool grid_ok(int64_t ctas) { return ctas < ((int64_t)1 << 31); }
-
 } // namespace mgpu_hip

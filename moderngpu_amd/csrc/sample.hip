@@ -39,7 +39,7 @@ int mgpu_hip_sample(const void* logits, int64_t logits_stride, int rows,
   if(out[0].overlaps(out[1])) return (int)hipErrorInvalidValue;
   size_t need = mgpu_hip_sample_workspace_bytes(rows, vocab);
   if(need && (!workspace || workspace_bytes < need ||
-    (uintptr_t)workspace % 8 || !detail::sample_grid_ok(rows, vocab)))
+    (uintptr_t)workspace % 8))
     return (int)hipErrorInvalidValue;
   return with_row_type(dtype, [&](auto* p) {
     return guarded(stream, [&](context_t& context) {

@@ -229,6 +229,28 @@ def test_strides_in_place_and_no_weights(dev, dtype):
     want.check_grad(grad, dtype)
 
 
+def test_empty_rows(dev):
+    """No logits at all: no teacher entry is usable."""
+    z = torch.empty(3, 0, device=dev)
+    ids, a = torch.zeros(3, 2, dtype=torch.int32, device=dev), torch.zeros(3, 2, device=dev)
+    loss, grad = m.distill_loss_and_grad(z, ids, a)
+    assert loss.tolist() == [0, 0, 0] and grad.shape == (3, 0)
+    loss, norms = m.distill_loss(z, ids, a)
+    assert loss.tolist() == [0, 0, 0] and not norms.any()
+
+
+def test_more_rows_than_one_launch(dev):
+    rows = (1 << 20) + 3
+    z = torch.zeros(rows, 4, device=dev)
+    z[-2, 1] = 2.0
+    ids = torch.ones(rows, 1, dtype=torch.int32, device=dev)
+    loss, grad = m.distill_loss_and_grad(z, ids, torch.zeros(rows, 1, device=dev))
+    flat, peak = math.log(4), math.log(3 + math.exp(2)) - 2
+    assert abs(loss[-1].item() - flat) < 1e-5 and abs(loss[-2].item() - peak) < 1e-5 and abs(loss[1 << 19].item() - flat) < 1e-5
+    assert (grad[-1].cpu() - torch.tensor([0.25, -0.75, 0.25, 0.25])).abs().max() < 1e-6
+    assert bool((loss[:-2] == loss[0]).all()) and bool((grad[:-2] == grad[0]).all())
+
+
 def test_leading_dimensions(dev):
     z, ids, teacher, weights = make(6, 100, 5, torch.float32)
     shape = lambda t: t.reshape((2, 3) + t.shape[1:]).to(dev)  # noqa: E731

@@ -154,6 +154,18 @@ def test_strides(dev, dtype):
     check(dev, z[:1].expand(5, 1001), u, view=one, p=0.8)
 
 
+def test_more_rows_than_go_together(dev):
+    """Rows past one round of launches, each with its own settings."""
+    rows = 20_011
+    z, u = logits(rows, 33, torch.float32, seed=16)
+    gen = torch.Generator().manual_seed(17)
+    k = torch.randint(0, 6, (rows,), generator=gen).to(torch.int32)
+    p = torch.rand(rows, generator=gen) * 1.2
+    t = torch.rand(rows, generator=gen) * 2
+    check(dev, z, u, t=t, k=k, p=p)
+    check(dev, z, u, least=torch.rand(rows, generator=gen) * 0.3)
+
+
 def test_ends_of_the_random_range(dev):
     """u = 0 takes the first kept token with a probability, the largest u
     below 1 the last; numbers outside [0, 1) count as the ends."""

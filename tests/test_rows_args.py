@@ -133,3 +133,20 @@ def test_python_layer_refuses():
         m.distill_loss(t, ids, t)
     with pytest.raises(TypeError):
         m.sample(t, torch.zeros(4))
+
+
+def test_numbers_past_what_kernels_index_are_refused(mem):
+    """Rows at one address (stride 0) take no memory, so these sizes can be
+    asked for; loops over a row would pass the largest int."""
+    _, p = mem
+    L = m.lib()
+    big = (1 << 30) + 1
+    assert L.mgpu_hip_embedding_lookup(p[0], 1, big, 0, p[1], 1, 1.0, p[2] + (1 << 40), big, F32, None) == INVALID
+    for n, rows, dim in ((big, 1, 1), (1, big, 1), (1, 1, big)):
+        assert L.mgpu_hip_embedding_grad_workspace_bytes(n, rows, dim) == 0
+        assert L.mgpu_hip_embedding_grad(p[0], 0, p[1], n, rows, dim, 1.0, 0, p[2] + (1 << 40), dim, F32, F32,
+                                         p[3], 1 << 62, None) == INVALID
+    assert L.mgpu_hip_distill_loss(p[0], 0, 1, big, p[1] + (1 << 40), p[2] + (1 << 40), 1, 1.0, None,
+                                   p[3] + (1 << 41), None, F32, F32, None) == INVALID
+    assert L.mgpu_hip_distill_grad(p[0], 0, 1, big, p[3], p[1], p[2], 1, 1.0, None, p[2] + (1 << 41), big, F32, F32,
+                                   None) == INVALID
