@@ -187,8 +187,11 @@ struct distill_f {
       if(id[j] >= 0 && a_max != -inf) a_sum += share(a[j], a_max);
     a_sum = join(a_max, a_sum, tid, shared_join[0]);
     if(a_max == -inf) {
-      if(!tid && loss) loss[row] = 0;
-      if(!tid && norms) norms[2 * (int64_t)row] = norms[2 * (int64_t)row + 1] = 0;
+      if(mode != distill_grad_only && !tid) {
+        loss[row] = 0;
+        if(norms)
+          norms[2 * (int64_t)row] = norms[2 * (int64_t)row + 1] = 0;
+      }
       if(mode != distill_loss_only) {
         chunk_t zero;
         PRAGMA_UNROLL

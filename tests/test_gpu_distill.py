@@ -229,6 +229,30 @@ def test_strides_in_place_and_no_weights(dev, dtype):
     want.check_grad(grad, dtype)
 
 
+def test_gradient_leaves_the_norms(dev):
+    """One loss, two gradients: a row that counts for nothing in the first
+    does in the second."""
+    gen = torch.Generator().manual_seed(21)
+    z = torch.randn(4, 300, generator=gen).to(dev)
+    ids = torch.randint(0, 300, (4, 5), generator=gen).to(torch.int32).to(dev)
+    a = torch.randn(4, 5, generator=gen).to(dev)
+    loss, norms = m.distill_loss(z, ids, a)
+    kept = norms.clone()
+    want = m.distill_grad(z, norms, ids, a)
+    none = m.distill_grad(z, norms, ids, a, weights=torch.tensor([0.0, 1, 0, 1], device=dev))
+    assert torch.equal(norms, kept)
+    assert not none[0].any() and not none[2].any()
+    assert torch.equal(m.distill_grad(z, norms, ids, a), want)
+
+
+def test_entries_without_dimensions_are_refused(dev):
+    z = torch.zeros(8, device=dev)
+    with pytest.raises(ValueError):
+        m.distill_loss(z, torch.tensor(1, dtype=torch.int32, device=dev), torch.tensor(0.0, device=dev))
+    loss, _ = m.distill_loss(z, torch.ones(1, dtype=torch.int32, device=dev), torch.zeros(1, device=dev))
+    assert abs(loss.item() - math.log(8)) < 1e-5
+
+
 def test_empty_rows(dev):
     """No logits at all: no teacher entry is usable."""
     z = torch.empty(3, 0, device=dev)
