@@ -157,7 +157,7 @@ def _distill_args(logits, teacher_ids, teacher_logits, weights):
     _int32(teacher_ids, "teacher_ids")
     if teacher_logits.dtype not in _ROW_DTYPES or not teacher_logits.is_cuda or not teacher_logits.is_contiguous():
         raise TypeError("teacher_logits must be a contiguous float32, float16 or bfloat16 CUDA tensor")
-    if teacher_ids.shape != teacher_logits.shape or teacher_ids.shape[:-1] != logits.shape[:-1]:
+    if not teacher_ids.dim() or teacher_ids.shape != teacher_logits.shape or teacher_ids.shape[:-1] != logits.shape[:-1]:
         raise ValueError("teacher_ids and teacher_logits must have a row for each row of logits")
     _same_device(logits.device, teacher_ids, teacher_logits)
     if weights is not None:
