@@ -77,7 +77,173 @@ struct embedding_lookup_f {
   }
 };
 
-// The gradient goes by the tokens in the order of their ids, three launches:
+// The gradient of few tokens: one launch in which a CTA takes `group_rows` rows
+// and `blocks` blocks of up to 64 chunks along them, looks at all ids, keeps
+// its own in LDS in the order of rows and tokens, and adds them up, a wave a
+// row.  Rows of more than `alone` tokens are shared out among the waves.  No
+// CTA waits for another's sort: the three launches below take 21.9 us for 1537
+// tokens into 10007 x 515 fp32 and 24.7 for 2048, this one 15.0 and 20.2 (bf16
+// into 1000 x 64: 28.9 and 11.2; 32768 x 1024: 25.8 and 23.3; 131072 x 4096:
+// 201 and 181).  A row of all 2048 tokens is where they are better (10007 x
+// 515: 24 against 68 us, one CTA's share of the memory): past 2048 they take
+// all.
+enum { embedding_few = 2048 };
+
+template<typename grad_t, typename out_t, bool stream>
+struct embedding_few_f {
+  enum { nt = 1024, waves = nt / 64, W = row_chunk_t<out_t>::width,
+    batch = 8, max_rows = 32, alone = 32, rounds = embedding_few / nt,
+    segments = embedding_few / 64 };
+  static_assert((int)max_rows * segments == nt, "a thread a row and segment");
+  typedef row_held_t<grad_t, W> held_t;
+  typedef row_held_t<out_t> held_out_t;
+  const grad_t* grad;
+  int64_t grad_stride;
+  const int* ids;
+  int count, num_rows, dim;
+  float scale;
+  int accumulate;
+  out_t* output;
+  int64_t output_stride;
+  int group_rows, cols, col_blocks, blocks, splits;
+  int first_cta;                // (of this launch)
+
+  __forceinline__ MGPU_DEVICE void write(int v, int col, const float (&sum)[W])
+    const {
+    out_t* p = output + v * output_stride + col;
+    float x[W];
+    PRAGMA_UNROLL
+    for(int j = 0; j < W; ++j) x[j] = scale * sum[j];
+    if(accumulate) {
+      held_out_t before;
+      before.load(p, dim - col, (out_t)0.f);
+      PRAGMA_UNROLL
+      for(int j = 0; j < W; ++j) x[j] += before.get(j);
+    }
+    row_store<stream>(x, p, dim - col);
+  }
+
+  // The sum of the tokens [begin, end) of the list.
+  __forceinline__ MGPU_DEVICE void add(const unsigned short* list, int begin,
+    int end, int col, float (&sum)[W]) const {
+    PRAGMA_UNROLL
+    for(int j = 0; j < W; ++j) sum[j] = 0;
+    if(col >= dim) return;
+    PRAGMA_NO_UNROLL
+    for(int i = begin; i < end; i += batch) {
+      held_t c[batch];
+      PRAGMA_UNROLL
+      for(int u = 0; u < batch; ++u)
+        if(i + u < end)
+          c[u].load(grad + list[i + u] * grad_stride + col, dim - col,
+            (grad_t)0.f);
+      PRAGMA_UNROLL
+      for(int u = 0; u < batch; ++u)
+        if(i + u < end) {
+          PRAGMA_UNROLL
+          for(int j = 0; j < W; ++j) sum[j] += c[u].get(j);
+        }
+    }
+  }
+
+  MGPU_DEVICE void operator()(int tid, int cta) const {
+    // Number, then place of the first, of each row's tokens in each segment
+    // of 64 tokens.
+    __shared__ int shared_at[nt + 1];
+    __shared__ int shared_scan[waves];
+    __shared__ unsigned short shared_list[embedding_few];
+    __shared__ float shared_sum[2][waves][W][64];
+    int wave = tid / 64, lane = tid & 63;
+    int v0 = (first_cta + cta / splits) * group_rows;
+    int rows = min(group_rows, num_rows - v0);
+
+    int r[rounds], rank[rounds];
+    bool any = false;
+    PRAGMA_UNROLL
+    for(int u = 0; u < rounds; ++u) {
+      int t = u * nt + tid;
+      int id = t < count ? ids[t] : -1;
+      r[u] = id >= v0 && id - v0 < rows ? id - v0 : -1;
+      any |= r[u] >= 0;
+    }
+    shared_at[tid] = 0;
+    if(!tid) shared_at[nt] = 0;
+    if(__syncthreads_count(any)) {
+      PRAGMA_UNROLL
+      for(int u = 0; u < rounds; ++u) {
+        lanemask_t peers = ballot(r[u] >= 0);
+        if(peers) {
+          PRAGMA_UNROLL
+          for(int b = 1; b < max_rows; b *= 2) {
+            lanemask_t set = ballot(r[u] & b);
+            peers &= r[u] & b ? set : ~set;
+          }
+        }
+        rank[u] = popc(peers & lanemask_lt(lane));
+        if(r[u] >= 0 && !(peers & ~lanemask_le(lane)))
+          shared_at[r[u] * segments + u * waves + wave] = rank[u] + 1;
+      }
+      __syncthreads();
+      int n = shared_at[tid];
+      int upto = wave_scan(n, plus_t<int>(), lane);
+      if(63 == lane) shared_scan[wave] = upto;
+      __syncthreads();
+      for(int w = 0; w < wave; ++w) upto += shared_scan[w];
+      shared_at[tid] = upto - n;
+      if(nt - 1 == tid) shared_at[nt] = upto;
+      __syncthreads();
+      PRAGMA_UNROLL
+      for(int u = 0; u < rounds; ++u)
+        if(r[u] >= 0)
+          shared_list[shared_at[r[u] * segments + u * waves + wave] + rank[u]] =
+            (unsigned short)(u * nt + tid);
+      __syncthreads();
+    } else if(accumulate) return;
+
+    int mine = min(lane, max_rows - 1) * segments;
+    lanemask_t shared_rows = ballot(lane < rows &&
+      shared_at[mine + segments] - shared_at[mine] > alone);
+    int first = cta % splits * blocks;
+    int joined = 0;
+    float sum[W];
+    for(int block = first; block < min(first + blocks, col_blocks); ++block) {
+      int col = lane < cols ? (block * cols + lane) * W : dim;
+      for(int i = wave; i < rows; i += waves) {
+        int begin = shared_at[i * segments], end = shared_at[(i + 1) * segments];
+        if(end - begin > alone || (accumulate && begin == end)) continue;
+        add(shared_list, begin, end, col, sum);
+        if(col < dim) write(v0 + i, col, sum);
+      }
+      for(lanemask_t rest = shared_rows; rest; rest &= rest - 1) {
+        int i = ffs(rest) - 1;
+        int begin = shared_at[i * segments], end = shared_at[(i + 1) * segments];
+        int piece = div_up(end - begin, (int)waves);
+        add(shared_list, begin + wave * piece,
+          min(begin + (wave + 1) * piece, end), col, sum);
+        // Two buffers: the last joining wave has read its one before it came
+        // to the barrier that stands between.
+        float (&sums)[waves][W][64] = shared_sum[joined & 1];
+        PRAGMA_UNROLL
+        for(int j = 0; j < W; ++j) sums[wave][j][lane] = sum[j];
+        __syncthreads();
+        if(wave == joined % waves && col < dim) {
+          PRAGMA_UNROLL
+          for(int j = 0; j < W; ++j) sum[j] = sums[0][j][lane];
+          PRAGMA_NO_UNROLL
+          for(int w = 1; w < waves; ++w) {
+            PRAGMA_UNROLL
+            for(int j = 0; j < W; ++j) sum[j] += sums[w][j][lane];
+          }
+          write(v0 + i, col, sum);
+        }
+        ++joined;
+      }
+    }
+  }
+};
+
+// The gradient of more goes by the tokens in the order of their ids, in three
+// launches:
 //   embedding_plan_f    order[] = the tokens sorted by id, equal ids in token
 //                       order, and starts[v] = where row v's tokens begin
 //   embedding_sum_f     a CTA per few rows adds up each row's tokens and
@@ -461,13 +627,12 @@ struct embedding_workspace_t {
   int blocks;
   embedding_workspace_t(int count, int num_rows, int dim) {
     auto aligned = [](size_t n) { return (n + 255) / 256 * 256; };
-    // Rows with more tokens than a block need that many tokens.
-    blocks = count > embedding_block ?
-      div_up(count, (int)embedding_block) : 0;
+    blocks = div_up(count, (int)embedding_block);
     starts = 0;
     order = aligned(sizeof(int) * ((size_t)num_rows + 1));
     partials = order + aligned(sizeof(int) * (size_t)count);
     bytes = partials + 2 * sizeof(float) * (size_t)blocks * dim;
+    if(count <= embedding_few) bytes = 0;
   }
 };
 
@@ -482,6 +647,41 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
   bool accumulate, out_t* output, int64_t output_stride, void* workspace,
   context_t& context) {
   if(num_rows <= 0 || dim <= 0 || (accumulate && count <= 0)) return;
+  // (What is added to is read as well, and stays in the caches.)
+  bool stream = !accumulate &&
+    (int64_t)num_rows * dim * (int64_t)sizeof(out_t) >= row_stream_bytes;
+  auto either = [&](auto f) {
+    if(stream) f(std::true_type());
+    else f(std::false_type());
+  };
+  if(count <= embedding_few)
+    return either([&](auto stream) {
+      typedef embedding_few_f<grad_t, out_t, decltype(stream)::value> few_t;
+      int chunks = div_up(dim, (int)few_t::W);
+      int col_blocks = div_up(chunks, 64);
+      int cols = div_up(chunks, col_blocks);
+      // As many rows a CTA as leave 512 of them, two on each CU.  Blocks of
+      // columns side by side up to 2048 CTAs, then up to 4 one after the other
+      // for one look at the ids (131072 x 4096, bf16 and fp32 results: 181 and
+      // 337 us; with 2: 188 and 304, with 8 and 16: 183 and 411).
+      int group_rows = few_t::max_rows;
+      while(group_rows > 1 &&
+        (int64_t)div_up(num_rows, group_rows) * col_blocks < 512)
+        group_rows /= 2;
+      int row_ctas = div_up(num_rows, group_rows);
+      int splits = max(div_up(col_blocks, 4), min(col_blocks, 2048 / row_ctas));
+      int blocks = div_up(col_blocks, splits);
+      splits = div_up(col_blocks, blocks);
+      int most = max(embedding_grid / splits, 1);
+      for(int first = 0; first < row_ctas; first += most) {
+        few_t few { grad, grad_stride, ids, count, num_rows, dim, scale,
+          accumulate, output, output_stride, group_rows, cols, col_blocks,
+          blocks, splits, first };
+        cta_launch<few_t::nt>(few, min(row_ctas - first, most) * splits,
+          context);
+      }
+    });
+
   embedding_workspace_t ws(count, num_rows, dim);
   int* starts = (int*)((char*)workspace + ws.starts);
   int* order = (int*)((char*)workspace + ws.order);
@@ -491,7 +691,7 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
   cta_launch<embedding_plan_nt>(plan, div_up(num_rows,
     (int)embedding_plan_rows), context);
 
-  auto add_up = [&](auto stream) {
+  either([&](auto stream) {
     typedef embedding_sum_f<grad_t, out_t, decltype(stream)::value> sum_t;
     embedding_shape_t shape(dim, sum_t::W);
     // A group's tokens come one batch after the other: about 16 of them, and
@@ -508,24 +708,16 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
       cta_launch<embedding_nt>(sum, min(block_ctas + row_ctas - first, most) *
         shape.col_blocks, context);
     }
-  };
-  // (What is added to is read as well, and stays in the caches.)
-  if(!accumulate &&
-    (int64_t)num_rows * dim * (int64_t)sizeof(out_t) >= row_stream_bytes)
-    add_up(std::true_type());
-  else
-    add_up(std::false_type());
+  });
 
-  if(ws.blocks) {
-    typedef embedding_long_f<out_t> long_t;
-    int col_blocks = div_up(dim, (int)long_t::cta_cols);
-    int most = max(embedding_grid / col_blocks, 1);
-    for(int first = 0; first < ws.blocks; first += most) {
-      long_t join { num_rows, dim, scale, accumulate, output, output_stride,
-        ids, starts, order, partials, col_blocks, first };
-      cta_launch<embedding_nt>(join, min(ws.blocks - first, most) * col_blocks,
-        context);
-    }
+  typedef embedding_long_f<out_t> long_t;
+  int col_blocks = div_up(dim, (int)long_t::cta_cols);
+  int most = max(embedding_grid / col_blocks, 1);
+  for(int first = 0; first < ws.blocks; first += most) {
+    long_t join { num_rows, dim, scale, accumulate, output, output_stride,
+      ids, starts, order, partials, col_blocks, first };
+    cta_launch<embedding_nt>(join, min(ws.blocks - first, most) * col_blocks,
+      context);
   }
 }
 

@@ -178,6 +178,49 @@ def test_grad_is_the_same_every_time(dev):
             assert torch.equal(m.embedding_grad(grad, ids, num_rows=500), first)
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("count,rows,dim", [(2047, 40, 300), (2048, 7, 520), (2049, 7, 520), (2049, 9000, 130),
+                                            (100, 20000, 1100), (2048, 4100, 2063)])
+def test_grad_of_few_tokens_and_of_more(dev, count, rows, dim, accumulate):
+    """Around 2048 tokens, where one launch gives way to three; several blocks
+    of columns, side by side and one after the other; several rows of many
+    tokens next to each other; strides and padding for both."""
+    gen = torch.Generator().manual_seed(count + rows)
+    for gtype, otype in ((torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)):
+        ids = make_ids("mixed", count, rows, gen)
+        hot = torch.rand(count, generator=gen) < 0.5
+        ids[hot] = torch.randint(0, min(rows, 5), (int(hot.sum()),), generator=gen).to(torch.int32)
+        wide = torch.randn(count, dim + 3, generator=gen).to(gtype)
+        outer = torch.full((rows, dim + 5), 2.0, dtype=otype, device=dev)
+        out = outer[:, 1:1 + dim]
+        m.embedding_grad(wide.to(dev)[:, 3:], ids.to(dev), out=out, accumulate=accumulate)
+        total, size, n = grad_want(wide[:, 3:], ids, rows)
+        base = 2.0 if accumulate else 0.0
+        near(out, total + base, (n[:, None] + 2) * 2.0 ** -24 * (size + base), otype)
+        assert bool((outer[:, :1] == 2).all()) and bool((outer[:, 1 + dim:] == 2).all())
+
+
+@pytest.mark.parametrize("count", [300, 2100])
+def test_grad_in_a_graph(dev, count):
+    gen = torch.Generator().manual_seed(count)
+    grad, ids = torch.randn(count, 70, generator=gen).to(dev), make_ids("mixed", count, 90, gen).to(dev)
+    out = torch.zeros(90, 70, device=dev)
+    m.embedding_grad(grad, ids, out=out)                         # warm
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m.embedding_grad(grad, ids, out=out)
+        m.embedding_grad(grad, ids, out=out, accumulate=True)
+    for seed in (1, 2, 3):
+        new = make_ids("mixed", count, 90, torch.Generator().manual_seed(seed)).to(dev)
+        ids.copy_(new)
+        grad.mul_(-0.5)
+        graph.replay()
+        want = m.embedding_grad(grad, ids, num_rows=90)
+        m.embedding_grad(grad, ids, out=want, accumulate=True)
+        assert torch.equal(out, want)
+
+
 def test_gradient_against_differences(dev):
     """Moving one table value by h moves the weighted sum of the lookups by h
     times its gradient (the map is linear: exact up to the 64-bit reference's

@@ -135,6 +135,15 @@ def test_python_layer_refuses():
         m.sample(t, torch.zeros(4))
 
 
+def test_grad_refuses_a_small_workspace(mem):
+    _, p = mem
+    L = m.lib()
+    need = L.mgpu_hip_embedding_grad_workspace_bytes(5000, 8, 4)
+    assert need > 5000 * 4
+    for ws, nb in ((p[3], need - 1), (None, need), (p[3] + 2, need)):
+        assert L.mgpu_hip_embedding_grad(p[0], 4, p[5], 5000, 8, 4, 1.0, 0, p[2], 4, F16, F16, ws, nb, None) == INVALID
+
+
 def test_numbers_past_what_kernels_index_are_refused(mem):
     """Rows at one address (stride 0) take no memory, so these sizes can be
     asked for; loops over a row would pass the largest int."""
