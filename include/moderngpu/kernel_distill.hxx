@@ -30,6 +30,9 @@ enum distill_mode_t { distill_loss_only, distill_grad_only, distill_both };
 // registers between the pass that sums it and the pass that writes the
 // gradient, and is read once; its loads are all in flight while the teacher's
 // entries are dealt with.  What a longer row has behind that is read by both.
+// Bound by memory: 2048 x 131072 bf16 take 220 us and 4096 x 32768 102 with a
+// fifth masked, where copies of as many bytes take 208 and 94; the 15
+// instructions a logit fit behind that.
 // The gradient is streamed past the caches, which the rows being read need (2048
 // x 131072 bf16: 222 us against 243, 333 x 50021 fp32 in two calls: 40.5 against
 // 43.6; 4096 x 32768 bf16 with a fifth of the rows masked: 102 against 100).
@@ -336,9 +339,10 @@ void distill_launch(const type_t* logits, int64_t stride, int rows, int vocab,
     // on a CU.  Past 32768 16-bit values that is one row in all its registers,
     // and two rows of which each holds half are faster (2048 x 65536 bf16: 114
     // us against 191 with 1024 threads, x 131072: 242 against 280; two that
-    // hold a quarter: 121 and 272; all before the stores were streamed).  32-bit rows have half the arithmetic a
-    // byte, and one row held by 1024 threads does (1024 x 65536: 128 us
-    // against 133, x 131072: 254 against 289).
+    // hold a quarter: 121 and 272; all before the stores were streamed).
+    // 32-bit rows have half the arithmetic a byte, and one row held by 1024
+    // threads does (1024 x 65536: 128 us against 133, x 131072: 254 against
+    // 289).
     if(vocab <= 256 * 4 * W)
       return launch(distill_f<type_t, teacher_t, mode, 256, 4>());
     if(vocab <= 512 * 8 * W)

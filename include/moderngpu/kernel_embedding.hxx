@@ -37,6 +37,10 @@ inline bool embedding_count_ok(int n) { return n <= 1 << 30; }
 enum { embedding_grid = 1 << 18 };
 
 // A thread moves `unroll` chunks of as many tokens, all on their way at once.
+// Bound by memory: 16384 rows of 4096 bf16 take 34 us (42 without streamed
+// results, 51 with one token a thread besides), 134 MB of results and 60 MB of
+// distinct rows, where a copy of as many bytes takes 38.  16 rows take the 2.5
+// us of a launch.
 template<typename type_t, int unroll, bool stream>
 struct embedding_lookup_f {
   const type_t* table;
@@ -252,6 +256,9 @@ struct embedding_few_f {
 // A row of more than embedding_block tokens is left out by its own CTA; its
 // tokens are added up in blocks of that many by further CTAs of the second
 // launch, so that no CTA adds more than rows-per-CTA * embedding_block rows.
+// 16384 tokens into 65536 x 2048 bf16: 10 + 50 + 5 us, and a copy of the 67 MB
+// read and 268 MB written takes 65; two steps into 32768 x 4096 fp32 249 us
+// (193).  Blocks of 64 tokens leave the longest chains twice as long.
 
 enum { embedding_plan_nt = 1024, embedding_plan_rows = 512,
   embedding_block = 32 };
@@ -513,10 +520,14 @@ struct embedding_sum_f {
   __forceinline__ MGPU_DEVICE void store_partial(int slot, int col,
     const float (&sum)[W]) const {
     float* p = partials + slot * (int64_t)dim + col;
-    row_values_t<float, W> x;
+    enum { width = row_chunk_t<float>::width };
     PRAGMA_UNROLL
-    for(int j = 0; j < W; ++j) x.x[j] = sum[j];
-    x.store(p, dim - col);
+    for(int i = 0; i < W; i += width) {
+      float x[width];
+      PRAGMA_UNROLL
+      for(int j = 0; j < width; ++j) x[j] = sum[i + j];
+      row_store(x, p + i, dim - col - i);
+    }
   }
 };
 

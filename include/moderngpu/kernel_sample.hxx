@@ -505,7 +505,8 @@ struct sample_weigh_f {
 
     // No logit below this is in a bin up to `high`: most pieces and runs of a
     // peaked row have none, and are passed over.
-    float floor = m - (high + 1 + slack) / (2 * s.c2);
+    float floor = __builtin_fmaxf(m - (high + 1 + slack) / (2 * s.c2),
+      -3.402823466e38f);
     if(mine.max < floor) {
       if(tid < sample_segments) mine.runs[tid] = 0;
       if(!tid) {
@@ -524,7 +525,7 @@ struct sample_weigh_f {
       int n = 0;
       PRAGMA_UNROLL
       for(int i = 0; i < W; ++i) {
-        bool reaches = z[c * W + i] >= floor && z[c * W + i] > -inf;
+        bool reaches = z[c * W + i] >= floor;     // not -inf, which NaN is by now
         lanemask_t those = ballot(reaches);
         if(reaches) {
           int at = n + popc(those & lanemask_lt(lane));
@@ -581,6 +582,10 @@ struct sample_weigh_f {
 // temperature at which all are nearly equal), it reads the row again: a border
 // is bracketed by the counts per half octave, the tokens above the bracket are
 // added up, those inside are listed, and the border is found among them.
+// Bound by its chain of steps with a barrier between them: 15 us for a row of
+// 131072 bf16 with all settings, 19 for 256 rows with top-p, 36 where one of 33
+// rows of 50021 fp32 keeps a thousand.  (One CTA that selects digit by digit on
+// the whole row: 442 us for the first.)
 enum { sample_nt = 1024, sample_row_bins = 128 };
 
 // Which tokens are kept: those with a larger key, and of those with this one

@@ -55,14 +55,12 @@ struct row_chunk_t {
 
   type_t x[width];
 
-  MGPU_DEVICE void load_all(const type_t* p) {
-    row_words_t w = ((const any_words_t*)p)->w;
-    __builtin_memcpy(x, &w, 16);
-  }
   // The first n values; `rest` in the others.
   MGPU_DEVICE void load(const type_t* p, int n, type_t rest) {
-    if(n >= width) load_all(p);
-    else {
+    if(n >= width) {
+      row_words_t w = ((const any_words_t*)p)->w;
+      __builtin_memcpy(x, &w, 16);
+    } else {
       PRAGMA_UNROLL
       for(int i = 0; i < width; ++i) x[i] = i < n ? p[i] : rest;
     }
@@ -140,34 +138,6 @@ __forceinline__ MGPU_DEVICE void row_store(
   }
   ch.template store<stream>(p, n);
 }
-
-// `width` values of a row, in 16-byte moves where they fill some: the results
-// for a chunk of inputs of a narrower type.
-template<typename type_t, int width>
-struct row_values_t {
-  enum { W = row_chunk_t<type_t>::width };
-  static_assert(0 == width % W, "whole chunks");
-  type_t x[width];
-
-  MGPU_DEVICE void load(const type_t* p, int n) {
-    PRAGMA_UNROLL
-    for(int i = 0; i < width; i += W) {
-      row_chunk_t<type_t> c;
-      c.load(p + i, n - i, (type_t)0.f);
-      PRAGMA_UNROLL
-      for(int j = 0; j < W; ++j) x[i + j] = c.x[j];
-    }
-  }
-  MGPU_DEVICE void store(type_t* p, int n) const {
-    PRAGMA_UNROLL
-    for(int i = 0; i < width; i += W) {
-      row_chunk_t<type_t> c;
-      PRAGMA_UNROLL
-      for(int j = 0; j < W; ++j) c.x[j] = x[i + j];
-      c.store(p + i, n - i);
-    }
-  }
-};
 
 struct float_max_t {
   MGPU_HOST_DEVICE float operator()(float a, float b) const {
