@@ -369,7 +369,8 @@ MGPU_HIP_API int mgpu_hip_embedding_lookup(const void* table, int num_rows,
  * neither read nor written.  ids outside [0, num_rows) add to nothing.  The
  * order of the additions depends on the sizes and the ids alone.
  * output_dtype is grad_dtype or MGPU_F32.  Workspace:
- * mgpu_hip_embedding_grad_workspace_bytes (0 for sizes that are refused). */
+ * mgpu_hip_embedding_grad_workspace_bytes (0: none, as for up to 2048 ids, or
+ * sizes that are refused). */
 MGPU_HIP_API size_t mgpu_hip_embedding_grad_workspace_bytes(int count,
   int num_rows, int dim);
 MGPU_HIP_API int mgpu_hip_embedding_grad(const void* grad,

@@ -33,9 +33,10 @@ enum distill_mode_t { distill_loss_only, distill_grad_only, distill_both };
 // Bound by memory: 2048 x 131072 bf16 take 220 us and 4096 x 32768 102 with a
 // fifth masked, where copies of as many bytes take 208 and 94; the 15
 // instructions a logit fit behind that.
-// The gradient is streamed past the caches, which the rows being read need (2048
-// x 131072 bf16: 222 us against 243, 333 x 50021 fp32 in two calls: 40.5 against
-// 43.6; 4096 x 32768 bf16 with a fifth of the rows masked: 102 against 100).
+// The gradient is streamed past the caches, which the rows being read need
+// (2048 x 131072 bf16: 222 us against 243, 333 x 50021 fp32 in two calls: 40.5
+// against 43.6; 4096 x 32768 bf16 with a fifth of the rows masked: 102 against
+// 100).
 template<typename type_t, typename teacher_t, distill_mode_t mode, int nt_,
   int chunks>
 struct distill_f {
@@ -229,7 +230,8 @@ struct distill_f {
       int k = tid + j * nt;
       p[j] = id[j] >= 0 ? share(a[j], a_max) * inv_a : 0.f;
       total[j] = p[j];
-      if(mode != distill_loss_only && id[j] >= 0 && (look[j] || shared_twice[k])) {
+      if(mode != distill_loss_only && id[j] >= 0 &&
+        (look[j] || shared_twice[k])) {
         // The first of the entries with this index stands for all.
         float sum = 0;
         bool first = true;
@@ -305,7 +307,9 @@ struct distill_f {
         held[i].renew();
         if(v < vocab) write(held[i], dz, v, from, scale);
       }
-      walk(z, tid, [&](const held_t& ch, int v) { write(ch, dz, v, from, scale); });
+      walk(z, tid, [&](const held_t& ch, int v) {
+        write(ch, dz, v, from, scale);
+      });
       __syncthreads();
       PRAGMA_UNROLL
       for(int j = 0; j < entries; ++j)
