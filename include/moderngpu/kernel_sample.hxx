@@ -401,7 +401,7 @@ struct sample_scale_t {
 // come within rounding of it).  One CTA per piece adds up the tokens above, by
 // runs, and lists those in the border's bins.  Without top-p, what is within
 // reach of min-p counts as above.  256 rows of 131072 bf16 with top-p 0.95 take
-// 38 us, 47 with the exponentials where the tokens lie instead of next to each
+// 36 us, 47 with the exponentials where the tokens lie instead of next to each
 // other; 13 of them read the logits again, the rest are the chain from the
 // pieces' tables to the first token and the tokens' unpacking.
 template<typename type_t>
@@ -583,7 +583,7 @@ struct sample_weigh_f {
 // is bracketed by the counts per half octave, the tokens above the bracket are
 // added up, those inside are listed, and the border is found among them.
 // Bound by its chain of steps with a barrier between them: 15 us for a row of
-// 131072 bf16 with all settings, 19 for 256 rows with top-p, 36 where one of 33
+// 131072 bf16 with all settings, 19 for 256 rows with top-p, 31 where one of 33
 // rows of 50021 fp32 keeps a thousand.  (One CTA that selects digit by digit on
 // the whole row: 442 us for the first.)
 enum { sample_nt = 1024, sample_row_bins = 128 };
@@ -808,13 +808,18 @@ struct sample_row_f {
     some = some && less < sample_bins;
     if(!tid) shared.listed = 0;
     __syncthreads();
-    for(int p = tid / 64; p < pieces; p += num_waves) {
+    // A wave a piece; of few pieces, several waves each (33 rows of 50021 fp32,
+    // a thousand kept: 31 us for the launch, 37 with half the waves idle).
+    int each = max(num_waves / pieces, 1), lane = tid & 63;
+    for(int p = tid / 64 / each; p < pieces; p += num_waves / each) {
       int count = a.piece[p].listed;
       if(count > sample_list) {
-        if(!(tid & 63)) atomicAdd(&shared.listed, (int)sample_candidates + 1);
+        if(!lane) atomicAdd(&shared.listed, (int)sample_candidates + 1);
         break;
       }
-      for(int i = tid & 63; i - (tid & 63) < count; i += 64) {
+      for(int first = tid / 64 % each * 64; first < count;
+        first += 64 * each) {
+        int i = first + lane;
         int v = 0;
         unsigned key = 0;
         if(i < count) {
@@ -824,8 +829,8 @@ struct sample_row_f {
         bool in = i < count && (!some || top - sample_key_bin(key) <= less);
         lanemask_t mask = ballot(in);
         int base = 0;
-        if(!(tid & 63) && mask) base = atomicAdd(&shared.listed, popc(mask));
-        int at = readlane(base, 0) + popc(mask & lanemask_lt(tid & 63));
+        if(!lane && mask) base = atomicAdd(&shared.listed, popc(mask));
+        int at = readlane(base, 0) + popc(mask & lanemask_lt(lane));
         if(in && at < sample_candidates) {
           shared.key[at] = key;
           shared.index[at] = v;
