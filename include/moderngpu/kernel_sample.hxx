@@ -999,20 +999,7 @@ struct sample_row_f {
             atomicAdd(&shared.runs[(v + c * nt * W) >> bits], run);
         }
       }
-      int n = popc(in);
-      int at = wave_scan(n, plus_t<int>(), a.tid & 63);
-      int base = 0;
-      if(63 == (a.tid & 63) && at) base = atomicAdd(&shared.listed, at);
-      at += readlane(base, 63) - n;
-      PRAGMA_UNROLL
-      for(int i = 0; i < per_thread; ++i)
-        if(in >> i & 1) {
-          if(at < sample_candidates) {
-            shared.key[at] = sample_key((float)ch[i / W].x[i % W]);
-            shared.index[at] = v + i / W * nt * W + i % W;
-          }
-          ++at;
-        }
+      append(a, v, ch, in, shared);
     });
     sum = fold(sum, plus_t<mass_t>(), a.tid, shared.wave_mass);
     listed = shared.listed;
