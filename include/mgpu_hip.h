@@ -422,7 +422,8 @@ MGPU_HIP_API int mgpu_hip_distill_loss_and_grad(const void* logits,
  * the largest.  token[row] is the first index, in order of index, at which
  * the running sum of the kept p exceeds uniform[row] times their total;
  * logprob[row] is the logarithm of its share of that total.  temperature
- * <= 0 keeps the first alone.  -inf and NaN are never drawn, +inf counts as
+ * <= 0 (or NaN) keeps the first alone; NaN as top_p or min_p keeps
+ * everything.  -inf and NaN are never drawn, +inf counts as
  * the largest finite float; a row with nothing else gives token -1 and
  * logprob -inf.  Probabilities are summed as 64-bit whole numbers: the token
  * does not depend on the order of the sums.

@@ -8,6 +8,7 @@
 //           whose predecessors sum up to less than top_p, the first always,
 //   min-p   of those, every one whose probability is at least min_p times the
 //           largest (min_p above 1 counts as 1).
+// A NaN temperature counts as 0, and NaN as top_p or min_p keeps everything.
 // The token is the first, in order of index, at which the running sum of the
 // kept probabilities exceeds u times their total.  T = 0 takes the first.
 //
@@ -84,6 +85,16 @@ enum { sample_piece_nt = 256, sample_piece = 8192,
   sample_few = 256,             // largest that groups' maxima find them for
   sample_candidates = 16384 };  // candidates of a row that fit its list
 
+// What a setting asks for; the host's choice of launches and the kernels go by
+// the same.  NaN as top_p or min_p asks for nothing.
+MGPU_HOST_DEVICE bool sample_by_count(int k, int vocab) {
+  return k > 0 && k < vocab;
+}
+MGPU_HOST_DEVICE bool sample_by_mass(float p) { return p < 1; }
+MGPU_HOST_DEVICE float sample_least(float min_p) {
+  return min_p > 0 ? __builtin_fminf(min_p, 1.f) : 0.f;
+}
+
 // One row's settings.
 struct sample_row_t {
   double c;                     // log2(e) / T
@@ -127,12 +138,12 @@ struct sample_settings_t {
     float t = temperature ? temperature[r] : temperature_all;
     s.k = top_k ? top_k[r] : top_k_all;
     float p = top_p ? top_p[r] : top_p_all;
-    s.least = __builtin_fminf(min_p ? min_p[r] : min_p_all, 1.f);
+    s.least = sample_least(min_p ? min_p[r] : min_p_all);
     if(!(t > 0)) { t = 1; s.k = 1; }
     s.c = 1.4426950408889634 / (double)t;
     s.c2 = (float)__builtin_fmin(2 * s.c, 1.5e38);
-    s.by_count = s.k > 0 && s.k < vocab;
-    s.by_mass = p < 1;
+    s.by_count = sample_by_count(s.k, vocab);
+    s.by_mass = sample_by_mass(p);
     s.p = __builtin_fmaxf(p, 0.f);
     return s;
   }
@@ -1387,9 +1398,10 @@ void sample_launch(const type_t* logits, int64_t stride, int rows, int vocab,
   sample_scale_t scale { min(62 - bits, 50) };
   sample_piece_t* from = (sample_piece_t*)workspace;
   // Not where all rows are known to have top-k, or neither top-p nor min-p.
-  bool weighed = (settings.top_k || settings.top_k_all <= 0 ||
-    settings.top_k_all >= vocab) && (settings.top_p || settings.top_p_all < 1 ||
-    settings.min_p || settings.min_p_all > 0);
+  bool weighed =
+    (settings.top_k || !sample_by_count(settings.top_k_all, vocab)) &&
+    (settings.top_p || sample_by_mass(settings.top_p_all) || settings.min_p ||
+      sample_least(settings.min_p_all) > 0);
   for(int row = 0; row < rows; row += most) {
     int n = min(rows - row, most);
     sample_piece_f<type_t> look { logits, stride, vocab, pieces, settings,

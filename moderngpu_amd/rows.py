@@ -227,7 +227,8 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     ``uniform`` holds one float32 in [0, 1) a row.  Each setting is a number,
     or a tensor with one value a row (float32; int32 for top_k).  top_k <= 0,
     top_p >= 1 and min_p <= 0 keep everything; temperature <= 0 takes the
-    largest logit, the first of several.  A row of nothing but -inf and NaN
+    largest logit, the first of several; NaN settings count as 0 for the
+    temperature, and as not given otherwise.  A row of nothing but -inf and NaN
     gives token -1 and logprob -inf."""
     if logits.dim() != 2:
         raise TypeError("logits must be two-dimensional")

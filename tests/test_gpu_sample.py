@@ -208,3 +208,19 @@ def test_refusals(dev):
         m.sample(z, u, top_k=1 << 40)
     with pytest.raises(m.MgpuError):
         m.sample(z[:, :0], u)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nan_settings(dev, dtype):
+    """NaN, one for all rows or a row's own: the temperature counts as 0,
+    top_p and min_p as not given."""
+    z, u = logits(5, 3001, dtype, seed=18)
+    for given, meant in ((dict(t=math.nan), dict(t=0.0)), (dict(p=math.nan), dict()), (dict(least=math.nan), dict()),
+                         (dict(p=math.nan, least=math.nan), dict()), (dict(p=0.8, least=math.nan), dict(p=0.8)),
+                         (dict(k=40, least=math.nan), dict(k=40)), (dict(p=math.nan, least=0.1), dict(least=0.1)),
+                         (dict(t=math.nan, p=0.9, least=math.nan), dict(t=0.0))):
+        want = check(dev, z, u, **meant)
+        for value in (lambda v: v, lambda v: torch.full((5,), v, device=dev)):
+            token, _ = m.sample(z.to(dev), u.to(dev), temperature=value(given.get("t", 1.0)), top_k=given.get("k", 0),
+                                top_p=value(given.get("p", 1.0)), min_p=value(given.get("least", 0.0)))
+            assert token.tolist() == want, given
