@@ -328,13 +328,14 @@ void distill_launch(const type_t* logits, int64_t stride, int rows, int vocab,
     typedef decltype(k) f_t;
     // (A launch counts its threads in 32 bits.)
     const int most = 1 << 20;
-    for(int row = 0; row < rows; row += most) {
+    for(int row = 0, n; row < rows; row += n) {
+      n = min(rows - row, most);
       f_t f { logits + row * stride, stride, vocab,
         ids + row * (int64_t)top, teacher + row * (int64_t)top, top, tau,
         (float)(1.4426950408889634 / tau), weights ? weights + row : nullptr,
         loss ? loss + row : nullptr, norms ? norms + 2 * (int64_t)row : nullptr,
         grad ? grad + row * grad_stride : nullptr, grad_stride };
-      cta_launch<f_t::nt>(f, min(rows - row, most), context);
+      cta_launch<f_t::nt>(f, n, context);
     }
   };
   enum { W = row_chunk_t<type_t>::width };

@@ -29,9 +29,6 @@ struct embedding_shape_t {
   }
 };
 
-// Counts that the kernels below can index with.
-inline bool embedding_count_ok(int n) { return n <= 1 << 30; }
-
 // CTAs of one launch; more than that go in several (a launch counts its
 // threads in 32 bits).
 enum { embedding_grid = 1 << 18 };
@@ -295,7 +292,7 @@ struct embedding_plan_f {
     int v0 = cta * R;
     int rows = min((int)R, num_rows - v0);
 
-    // The wave's tokens (count <= 2^30, see embedding_count_ok).
+    // The wave's tokens (count <= 2^30, see row_count_ok).
     int piece = div_up(div_up(count, (int)W), 64) * 64;
     int begin = (int)min(wave * (int64_t)piece, (int64_t)count);
     int end = (int)min(begin + (int64_t)piece, (int64_t)count);

@@ -1402,8 +1402,8 @@ void sample_launch(const type_t* logits, int64_t stride, int rows, int vocab,
     (settings.top_k || !sample_by_count(settings.top_k_all, vocab)) &&
     (settings.top_p || sample_by_mass(settings.top_p_all) || settings.min_p ||
       sample_least(settings.min_p_all) > 0);
-  for(int row = 0; row < rows; row += most) {
-    int n = min(rows - row, most);
+  for(int row = 0, n; row < rows; row += n) {
+    n = min(rows - row, most);
     sample_piece_f<type_t> look { logits, stride, vocab, pieces, settings,
       from };
     cta_launch<sample_piece_nt>(look, n * pieces, context);

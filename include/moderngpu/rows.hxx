@@ -20,6 +20,10 @@ typedef __bf16 bf16_t;
 
 namespace detail {
 
+// Numbers of tokens and rows, and of values of a row, that the entry points
+// take: the kernels' own sums of them with a tile or a grid stay below 2^31.
+inline bool row_count_ok(int n) { return n <= 1 << 30; }
+
 typedef unsigned row_words_t __attribute__((ext_vector_type(4)));
 // The same 16 bytes at an address that is aligned to 2 or 4 of them only (an
 // alignment on a typedef would be dropped where it goes through a template).

@@ -23,8 +23,9 @@ struct distill_args_t {
 
   bool ok() const {
     size_t value = row_value_size(dtype), tv = row_value_size(teacher_dtype);
-    return value && tv && rows >= 0 && vocab >= 0 &&
-      vocab <= distill_max_vocab && top >= 0 && top <= distill_max_top && tau > 0 && tau < __builtin_inff() &&
+    return value && tv && rows >= 0 && detail::row_count_ok(rows) &&
+      vocab >= 0 && vocab <= distill_max_vocab && top >= 0 &&
+      top <= distill_max_top && tau > 0 && tau < __builtin_inff() &&
       1.4426950408889634 / tau < 3e38 && (double)tau * tau < 3e38 &&
       logit().input_ok() && id().input_ok() && entry().input_ok() &&
       weight().input_ok();

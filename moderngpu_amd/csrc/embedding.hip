@@ -18,7 +18,7 @@ int mgpu_hip_embedding_lookup(const void* table, int num_rows, int dim,
   matrix_t out(output, count, dim, output_stride, value);
   if(!in.input_ok() || !id.input_ok() || !out.output_ok() ||
     out.overlaps(in) || out.overlaps(id) ||
-    !detail::embedding_count_ok(count) || !detail::embedding_count_ok(dim))
+    !detail::row_count_ok(count) || !detail::row_count_ok(dim))
     return (int)hipErrorInvalidValue;
   return with_row_type(dtype, [&](auto* p) {
     typedef std::remove_pointer_t<decltype(p)> type_t;
@@ -32,9 +32,9 @@ int mgpu_hip_embedding_lookup(const void* table, int num_rows, int dim,
 size_t mgpu_hip_embedding_grad_workspace_bytes(int count, int num_rows,
   int dim) {
   if(count < 0 || num_rows < 0 || dim < 0 ||
-    !detail::embedding_count_ok(count) ||
-    !detail::embedding_count_ok(num_rows) ||
-    !detail::embedding_count_ok(dim)) return 0;
+    !detail::row_count_ok(count) ||
+    !detail::row_count_ok(num_rows) ||
+    !detail::row_count_ok(dim)) return 0;
   return detail::embedding_grad_workspace_bytes(count, num_rows, dim);
 }
 
@@ -53,8 +53,8 @@ int mgpu_hip_embedding_grad(const void* grad, int64_t grad_stride,
   matrix_t out(output, num_rows, dim, output_stride, out_value);
   if(!in.input_ok() || !id.input_ok() || !out.output_ok() ||
     out.overlaps(in) || out.overlaps(id) ||
-    !detail::embedding_count_ok(count) ||
-    !detail::embedding_count_ok(num_rows) || !detail::embedding_count_ok(dim))
+    !detail::row_count_ok(count) ||
+    !detail::row_count_ok(num_rows) || !detail::row_count_ok(dim))
     return (int)hipErrorInvalidValue;
   size_t need = mgpu_hip_embedding_grad_workspace_bytes(count, num_rows, dim);
   if(need && (!workspace || workspace_bytes < need ||

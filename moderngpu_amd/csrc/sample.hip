@@ -11,7 +11,8 @@ static_assert((int)MGPU_HIP_SAMPLE_MAX_VOCAB == (int)sample_max_vocab,
 extern "C" {
 
 size_t mgpu_hip_sample_workspace_bytes(int rows, int vocab) {
-  if(rows < 0 || vocab < 1 || vocab > sample_max_vocab) return 0;
+  if(rows < 0 || !detail::row_count_ok(rows) || vocab < 1 ||
+    vocab > sample_max_vocab) return 0;
   return detail::sample_workspace_bytes(rows, vocab);
 }
 
@@ -21,8 +22,8 @@ int mgpu_hip_sample(const void* logits, int64_t logits_stride, int rows,
   int top_k_all, float top_p_all, float min_p_all, int* token, float* logprob,
   int dtype, void* workspace, size_t workspace_bytes, mgpu_stream_t stream) {
   size_t value = row_value_size(dtype);
-  if(!value || rows < 0 || vocab < 1 || vocab > sample_max_vocab)
-    return (int)hipErrorInvalidValue;
+  if(!value || rows < 0 || !detail::row_count_ok(rows) || vocab < 1 ||
+    vocab > sample_max_vocab) return (int)hipErrorInvalidValue;
   auto column = [&](const void* p, bool there) {
     return matrix_t(p, there ? rows : 0, 1, 1, 4);
   };

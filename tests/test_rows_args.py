@@ -159,3 +159,19 @@ def test_numbers_past_what_kernels_index_are_refused(mem):
                                    p[3] + (1 << 41), None, F32, F32, None) == INVALID
     assert L.mgpu_hip_distill_grad(p[0], 0, 1, big, p[3], p[1], p[2], 1, 1.0, None, p[2] + (1 << 41), big, F32, F32,
                                    None) == INVALID
+
+
+def test_numbers_of_rows_past_2_30_are_refused(mem):
+    """One row of logits for all (stride 0) is small; a counter of rows that
+    go launch by launch would pass the largest int."""
+    _, p = mem
+    L = m.lib()
+    far = lambda i: p[0] + (i << 40)  # noqa: E731
+    for rows in ((1 << 30) + 1, (1 << 31) - 1):
+        teacher = (far(1), far(2), 1, 1.0, None)
+        assert L.mgpu_hip_distill_loss(p[0], 0, rows, 1, *teacher, far(3), far(4), F32, F32, None) == INVALID
+        assert L.mgpu_hip_distill_grad(p[0], 0, rows, 1, far(4), *teacher, far(5), 1, F32, F32, None) == INVALID
+        assert L.mgpu_hip_distill_loss_and_grad(p[0], 0, rows, 1, *teacher, far(3), far(5), 1, F32, F32, None) == INVALID
+        assert L.mgpu_hip_sample_workspace_bytes(rows, 1) == 0
+        assert L.mgpu_hip_sample(p[0], 0, rows, 1, far(1), None, None, None, None, 1.0, 0, 1.0, 0.0, far(2), far(3),
+                                 F32, p[1], 1 << 40, None) == INVALID
