@@ -324,6 +324,7 @@ void distill_launch(const type_t* logits, int64_t stride, int rows, int vocab,
   const float* weights, float* loss, float* norms, type_t* grad,
   int64_t grad_stride, context_t& context) {
   if(rows <= 0) return;
+  row_require(vocab <= distill_max_vocab && top <= distill_max_top);
   auto launch = [&](auto k) {
     typedef decltype(k) f_t;
     // (A launch counts its threads in 32 bits.)
@@ -362,7 +363,8 @@ void distill_launch(const type_t* logits, int64_t stride, int rows, int vocab,
 
 // loss[row], and norms[2 * row], norms[2 * row + 1] = the row's largest logit
 // and the logarithm of sum exp((z - largest) / tau), for distill_grad.
-// weights may be null (all 1); norms may be null.
+// weights may be null (all 1); norms may be null.  Up to distill_max_top
+// entries and distill_max_vocab logits a row; more throws, here and below.
 template<typename type_t, typename teacher_t>
 void distill_loss(const type_t* logits, int64_t stride, int rows, int vocab,
   const int* ids, const teacher_t* teacher, int top, float tau,

@@ -595,12 +595,13 @@ struct embedding_long_f {
 
 // output[t] = scale * table[ids[t]], t in [0, count), each value rounded once
 // from the 32-bit product.  table has num_rows rows of dim values, row_stride
-// values from one start to the next.
+// values from one start to the next.  count and dim up to 2^30.
 template<typename type_t>
 void embedding_lookup(const type_t* table, int num_rows, int dim,
   int64_t row_stride, const int* ids, int count, float scale, type_t* output,
   int64_t output_stride, context_t& context) {
   if(count <= 0 || dim <= 0) return;
+  detail::row_require(detail::row_count_ok(count) && detail::row_count_ok(dim));
   detail::embedding_shape_t shape(dim, detail::row_chunk_t<type_t>::width);
   auto launch = [&](auto unroll, auto stream) {
     enum { tokens = decltype(unroll)::value };
@@ -735,10 +736,14 @@ void embedding_grad_launch(const grad_t* grad, int64_t grad_stride,
 // row v, or with accumulate output[v] += that for the rows that occur (the
 // others are not touched).  Sums run in 32 bits in an order that depends on
 // the ids alone; the result, with what was there before, is rounded once.
+// count, num_rows and dim up to 2^30.
 template<typename grad_t, typename out_t>
 void embedding_grad(const grad_t* grad, int64_t grad_stride, const int* ids,
   int count, int num_rows, int dim, float scale, bool accumulate,
   out_t* output, int64_t output_stride, context_t& context) {
+  if(num_rows <= 0 || dim <= 0 || (accumulate && count <= 0)) return;
+  detail::row_require(detail::row_count_ok(count) &&
+    detail::row_count_ok(num_rows) && detail::row_count_ok(dim));
   mem_t<char> workspace(detail::embedding_grad_workspace_bytes(count,
     num_rows, dim), context);
   detail::embedding_grad_launch(grad, grad_stride, ids, count, num_rows, dim,

@@ -1424,8 +1424,8 @@ void sample_launch(const type_t* logits, int64_t stride, int rows, int vocab,
 } // namespace detail
 
 // token[row] and logprob[row] (its log probability among the kept ones) for
-// `rows` rows of `vocab` logits, vocab in [1, sample_max_vocab].  uniform: one
-// number in [0, 1) a row.  The settings are one value a row, or, where the
+// `rows` rows of `vocab` logits, vocab in [1, sample_max_vocab] (others throw).
+// uniform: one number in [0, 1) a row.  The settings are one value a row, or, where the
 // pointer is null, the same for all.  A row with nothing to draw gives token
 // -1 and logprob -inf.
 template<typename type_t>
@@ -1434,6 +1434,8 @@ void sample(const type_t* logits, int64_t stride, int rows, int vocab,
   const float* top_p, const float* min_p, float temperature_all,
   int top_k_all, float top_p_all, float min_p_all, int* token, float* logprob,
   context_t& context) {
+  if(rows <= 0) return;
+  detail::row_require(vocab >= 1 && vocab <= sample_max_vocab);
   mem_t<char> workspace(detail::sample_workspace_bytes(rows, vocab), context);
   detail::sample_launch(logits, stride, rows, vocab, uniform,
     detail::sample_settings_t { temperature, top_k, top_p, min_p,

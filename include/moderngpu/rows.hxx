@@ -23,6 +23,10 @@ namespace detail {
 // Numbers of tokens and rows, and of values of a row, that the entry points
 // take: the kernels' own sums of them with a tile or a grid stay below 2^31.
 inline bool row_count_ok(int n) { return n <= 1 << 30; }
+// The templates throw where the C entry points return an error.
+inline void row_require(bool ok) {
+  if(!ok) throw cuda_exception_t(hipErrorInvalidValue);
+}
 
 typedef unsigned row_words_t __attribute__((ext_vector_type(4)));
 // The same 16 bytes at an address that is aligned to 2 or 4 of them only (an
