@@ -111,6 +111,14 @@ struct sample_row_t {
   __forceinline__ MGPU_DEVICE static int bin(float quarters) {
     return (int)__builtin_floorf(quarters);
   }
+  // Whether the sums by quarter octaves around a logit at q of them hold what
+  // their bins say.  Floats below 2^25 lie 2 apart or less, so that a product
+  // is off by 1, and a difference of two bins' numbers by 3 with the digits cut
+  // off; past that they lie up to 16 apart.  (Temperatures below 2e-38 have
+  // bins that are too wide.)
+  __forceinline__ MGPU_DEVICE bool by_bins(float q) const {
+    return __builtin_fabsf(q) + 4 * sample_bins < 33554432.f && c2 < 1.5e38f;
+  }
   // top-k: whether the row has to drop candidates of some pieces for others'.
   __forceinline__ MGPU_DEVICE bool counted(int pieces) const {
     return k > sample_few || k * pieces > sample_candidates / 2;
@@ -362,7 +370,8 @@ struct sample_piece_f {
         part += e;
         if(!all) {
           // In a measure of the bin's octave, so that 24 bits do: no column
-          // gets past 128 * 2^24.
+          // gets past 128 * 2^24 where the table is looked at (see by_bins:
+          // 3 quarters too far down make 2^23.75 of a probability).
           int down = top - sample_row_t::bin(s.quarters(z[i]));
           if(down < sample_bins)
             atomicAdd(&shared_table[down][lane], (unsigned)
@@ -410,8 +419,11 @@ struct sample_scale_t {
 // Second launch, for rows with top-p or min-p but no top-k: with the sums of
 // all its pieces, a row's border lies in one quarter octave (two, should a sum
 // come within rounding of it).  One CTA per piece adds up the tokens above, by
-// runs, and lists those in the border's bins.  Without top-p, what is within
-// reach of min-p counts as above.  256 rows of 131072 bf16 with top-p 0.95 take
+// runs, and lists those in the border's bins.  Rows that are too many quarter
+// octaves away from zero for their bins' numbers (logits past 10^7 or a
+// temperature below 10^-6, say) have every token listed that has a probability
+// left: few at such temperatures.  Without top-p, what is within reach of min-p
+// counts as above.  256 rows of 131072 bf16 with top-p 0.95 take
 // 36 us, 47 with the exponentials where the tokens lie instead of next to each
 // other; 13 of them read the logits again, the rest are the chain from the
 // pieces' tables to the first token and the tokens' unpacking.
@@ -454,11 +466,11 @@ struct sample_weigh_f {
     // Far from zero the bins' numbers are rounded: by 2^-24 of them, twice.
     float q = s.quarters(m), far = __builtin_fabsf(q) + 4 * sample_bins;
     int top = sample_row_t::bin(q), slack = 1 + (int)(3e-7f * far);
-    int low = 0x7fffffff, high = 4 * scale.nothing_left();
+    int low = s.by_mass ? 0 : 0x7fffffff, high = 4 * scale.nothing_left();
     if(s.least > 0)
       high = min(high, (int)(-4 * __builtin_amdgcn_logf((float)s.least)));
     high += slack;
-    if(s.by_mass) {
+    if(s.by_mass && s.by_bins(q)) {
       double sum = 0;
       for(int p = tid; p < pieces; p += nt)
         if(of_row[p].max > -inf)
@@ -1094,8 +1106,9 @@ struct sample_row_f {
     sample_cut_t cut = { 0, vocab };
     if(a.s.by_mass) {
       above = fold(above, plus_t<mass_t>(), a.tid, shared.wave_mass);
-      cut = border_of(a, n, true, cut, goal(a.s.p * sum * scale.one()) - above,
-        shared);
+      mass_t want = goal(a.s.p * sum * scale.one());
+      // (What is above comes from sums by bins, the goal from another sum.)
+      cut = border_of(a, n, true, cut, max(want, above + 1) - above, shared);
     }
     __syncthreads();
     draw_from_runs(a, n, cut, shared);

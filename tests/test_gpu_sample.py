@@ -224,3 +224,37 @@ def test_nan_settings(dev, dtype):
             token, _ = m.sample(z.to(dev), u.to(dev), temperature=value(given.get("t", 1.0)), top_k=given.get("k", 0),
                                 top_p=value(given.get("p", 1.0)), min_p=value(given.get("least", 0.0)))
             assert token.tolist() == want, given
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_logits_many_temperatures_from_zero(dev, dtype):
+    """Logits a few steps of the type apart that lie 10^7 temperatures and more
+    from zero: the products logit / temperature are further apart than 1."""
+    step = lambda a: 2.0 ** (math.frexp(a)[1]) * torch.finfo(dtype).eps / 2  # noqa: E731
+    for vocab in (8192, 20011):
+        for a in (23300014.0, 15.1, 2000000.0, -15.1, 1.7):
+            a = torch.tensor(a).clamp(max=60000.0 if dtype == torch.float16 else 1e9).to(dtype).item()
+            for steps, share in ((3, 1 / 6), (4, 0.17), (2, 0.3), (1, 1.0)):
+                z = torch.full((3, vocab), a - steps * step(a)).to(dtype)
+                z[:, 0] = a
+                z[1, ::3] = a - (steps + 1) * step(a)
+                z[2, ::7] = -math.inf
+                u = torch.tensor([0.9871234, 0.31, 0.6])
+                t = float(np.float32(steps * step(a) * share))
+                for settings in (dict(p=0.5), dict(p=0.9), dict(least=0.001), dict(p=0.9, least=0.001), dict()):
+                    check(dev, z, u, t=t, **settings)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_temperatures_next_to_zero(dev, dtype):
+    """Temperatures that leave a few tokens; logits among the smallest numbers
+    with a temperature among them."""
+    z, u = logits(4, 20011, dtype, seed=20)
+    for t in (1e-3, 1e-5, 1e-6, 1e-8, 1e-20, 1e-38, 1e-45):
+        for settings in (dict(p=0.95), dict(p=0.5, least=0.1), dict(least=0.3), dict(k=50, p=0.9), dict()):
+            check(dev, z, u, t=t, **settings)
+    if dtype != torch.float16:
+        small = (z.double() * 4e-39).to(dtype)
+        for t in (1e-38, 1.8e-38, 1.2e-38):
+            for settings in (dict(p=0.3), dict(p=0.95), dict(least=0.01, p=0.7), dict(k=30), dict()):
+                check(dev, small, u, t=t, **settings)
