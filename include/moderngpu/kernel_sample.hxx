@@ -1132,24 +1132,23 @@ struct sample_row_f {
     if(!a.tid) done(a, (int)v, (double)total / scale.one());
   }
 
-  // One reading of the row per border (and one for the total between top-k and
-  // top-p); the last one leaves what the draw needs.  sum: top-p's without
-  // top-k.
+  // Rows with top-k or top-p (min-p alone lists nothing and comes from the
+  // second launch).  One reading of the row per border (and one for the total
+  // between top-k and top-p); the last one leaves what the draw needs.  sum:
+  // top-p's without top-k.
   __forceinline__ MGPU_DEVICE void on_the_row(const at_t& a, float reach,
     double sum, shared_t& shared) const {
-    enum { border_by_count, total, border_by_mass, min_p_alone };
+    enum { border_by_count, total, border_by_mass };
     sample_cut_t cut = { 0, vocab };
     float low = -1;
     int n = 0;
     bool again = false;
     PRAGMA_NO_UNROLL
-    for(int step = border_by_count; step <= min_p_alone; ++step) {
+    for(int step = border_by_count; step <= border_by_mass; ++step) {
       bool by_mass = step != border_by_count;
-      if(min_p_alone == step ? a.s.by_count || a.s.by_mass :
-        (step <= total && !a.s.by_count) || (by_mass && !a.s.by_mass)) continue;
+      if((step <= total && !a.s.by_count) || (by_mass && !a.s.by_mass)) continue;
       float high = nothing_left();
       if(total == step) low = __builtin_inff();
-      else if(min_p_alone == step) high = reach;
       else {
         count_row(a, shared);
         float down;
@@ -1158,13 +1157,6 @@ struct sample_row_f {
         high = __builtin_fminf(down, by_mass || !a.s.by_mass ? reach : high);
       }
       mass_t above = add_above(a, by_mass, cut, low, high, n, shared);
-      if(min_p_alone == step) {
-        if(n > sample_candidates) {
-          low = __builtin_inff();
-          add_above(a, by_mass, cut, low, high, n, shared);
-        }
-        break;
-      }
       if(total == step) {
         sum = (double)above / scale.one();
         continue;
