@@ -281,3 +281,88 @@ def test_refusals(dev):
         m.embedding_grad(t, ids, out=torch.zeros(1, 6, device=dev).expand(4, 6))
     with pytest.raises(m.MgpuError):
         m.embedding_grad(t, ids, out=t)
+
+
+# ---- sizes at which other kernels, or more launches, take over ----------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count,dim", [(16501, 1021), (17003, 2051), (8195, 4099), (140001, 33)])
+def test_lookup_of_many_tokens(dev, dtype, count, dim):
+    """Four tokens a thread, results below 64 MB and streamed ones, rows that
+    begin off every boundary."""
+    gen = torch.Generator().manual_seed(count)
+    table = torch.randn(777, dim + 1, generator=gen).to(dtype)
+    ids = make_ids("mixed", count, 777, gen)
+    ids[::3] = torch.randint(0, 777, ids[::3].shape, generator=gen).to(torch.int32)
+    out = torch.full((count, dim + 3), 5.0, dtype=dtype, device=dev)
+    m.embedding_lookup(table.to(dev)[:, 1:], ids.to(dev), scale=1.75, out=out[:, 1:1 + dim])
+    near(out[:, 1:1 + dim], *(lambda w: (w, w.abs() * 2.0 ** -24))(lookup_want(table[:, 1:], ids, 1.75)), dtype)
+    assert bool((out[:, 0] == 5).all()) and bool((out[:, 1 + dim:] == 5).all())
+
+
+def test_lookup_in_several_launches(dev):
+    """Tokens past one launch of 2^18 CTAs, by their number and by the length
+    of their rows.  Every value is compared, on the device (the products are
+    exact)."""
+    for count, dim, rows in ((2 ** 25 + 77, 3, 1000), (2051, 2 ** 20 + 8, 5)):
+        gen = torch.Generator(device=dev).manual_seed(dim)
+        table = torch.randn(rows, dim, generator=gen, device=dev).to(torch.bfloat16)
+        ids = torch.randint(-1, rows, (count,), generator=gen, device=dev, dtype=torch.int32)
+        out = m.embedding_lookup(table, ids, scale=2.0)
+        want = torch.cat([table * 2, torch.zeros(1, dim, dtype=table.dtype, device=dev)])
+        for begin in range(0, count, 2 ** 22 if dim == 3 else 512):
+            part = ids[begin:begin + (2 ** 22 if dim == 3 else 512)].long()
+            assert torch.equal(out[begin:begin + part.numel()], want[part])
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("types", [(t, t) for t in TYPES] + [(torch.bfloat16, torch.float32)], ids=lambda t: "%s-%s" % t)
+@pytest.mark.parametrize("count,rows,dim", [(2501, 16411, 2051), (1501, 16411, 2051), (20011, 9001, 130)])
+def test_grad_of_large_tables(dev, count, rows, dim, types, accumulate):
+    """Results of 64 MB and more, from few tokens and from many; more tokens
+    than the sort keeps between its passes.  Rows of many tokens among them."""
+    gtype, otype = types
+    gen = torch.Generator().manual_seed(count)
+    ids = make_ids("mixed", count, rows, gen)
+    ids[::5] = torch.randint(0, rows, ids[::5].shape, generator=gen).to(torch.int32)
+    ids[1::5] = 7
+    grad = torch.randn(count, dim, generator=gen).to(gtype)
+    out = torch.full((rows, dim), 2.0, dtype=otype, device=dev)
+    m.embedding_grad(grad.to(dev), ids.to(dev), scale=0.75, out=out, accumulate=accumulate)
+    # what occurs, in 64 bits; the other rows hold zeros, or what they held
+    used = torch.unique(ids[(ids >= 0) & (ids < rows)])
+    place = torch.full((rows,), -1, dtype=torch.int64)
+    place[used.long()] = torch.arange(used.numel())
+    inside = (ids >= 0) & (ids < rows)
+    local = torch.where(inside, place[ids.long().clamp(0, rows - 1)], -1)
+    total, size, n = grad_want(grad, local, used.numel())
+    base = 2.0 if accumulate else 0.0
+    near(out[used.long().to(dev)], base + 0.75 * total, (n[:, None] + 2) * 2.0 ** -24 * (base + 0.75 * size), otype)
+    rest = torch.ones(rows, dtype=torch.bool, device=dev)
+    rest[used.long().to(dev)] = False
+    assert bool((out[rest] == base).all())
+
+
+def test_grad_in_several_launches(dev):
+    """Rows and blocks of tokens past one launch of 2^18 CTAs: of few tokens by
+    the rows, of many by the rows, the blocks and the length of a row.  Whole
+    numbers, whose sums are exact; every value is compared, on the device."""
+    for count, rows, dim, repeat in ((1500, 2 ** 23 + 999, 2, False),            # one launch's kernel
+                                     (5000, 2 ** 26 + 5000, 1, False),           # sums, by rows
+                                     (2 ** 23 + 12345, 50, 1, False),            # joins, by blocks
+                                     (20000, 40, 2 ** 19 + 4, True)):            # both, by columns
+        gen = torch.Generator(device=dev).manual_seed(count)
+        ids = torch.randint(-1, rows, (count,), generator=gen, device=dev, dtype=torch.int32)
+        ids[::3] = rows - 1
+        grad = torch.randint(-4, 5, (1 if repeat else count, dim), generator=gen, device=dev).float()
+        ok = ids >= 0
+        at = ids[ok].long()
+        if repeat:                  # one gradient row for all tokens
+            want = torch.bincount(at, minlength=rows).float()[:, None] * grad
+            grad = grad.expand(count, dim)
+        else:
+            want = torch.stack([torch.bincount(at, weights=grad[ok, j].double(), minlength=rows) for j in range(dim)], 1).float()
+        out = m.embedding_grad(grad, ids, num_rows=rows)
+        assert torch.equal(out, want), (count, rows, dim)
+        m.embedding_grad(grad, ids, out=out, accumulate=True)
+        assert torch.equal(out, 2 * want), (count, rows, dim)
