@@ -258,3 +258,40 @@ def test_temperatures_next_to_zero(dev, dtype):
         for t in (1e-38, 1.8e-38, 1.2e-38):
             for settings in (dict(p=0.3), dict(p=0.95), dict(least=0.01, p=0.7), dict(k=30), dict()):
                 check(dev, small, u, t=t, **settings)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [270001, 600001])
+def test_wide_vocabularies(dev, dtype, vocab):
+    """More than 64 pieces, and runs of more than 64 chunks; candidates for a k
+    of 256 that outdo each other across pieces."""
+    z, u = logits(2, vocab, dtype, seed=22)
+    z[1, ::5] = -math.inf
+    for settings in (dict(), dict(p=0.95), dict(p=0.9, least=0.001), dict(least=0.01), dict(k=256), dict(k=256, p=0.9),
+                     dict(k=1536), dict(k=5000, p=0.99), dict(t=2.0, p=0.999), dict(t=0.0)):
+        check(dev, z, u, **settings)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ties_in_a_wide_vocabulary(dev, dtype):
+    """One value all through, and few values: a border is an index of three
+    digits."""
+    gen = torch.Generator().manual_seed(23)
+    z = torch.randint(-2, 3, (2, 600001), generator=gen).to(dtype)
+    z[0] = 0.5
+    u = torch.tensor([0.77, 0.99])
+    for settings in (dict(), dict(k=256), dict(k=450001), dict(p=0.7), dict(k=500000, p=0.4), dict(p=0.3, least=0.1), dict(t=0.0)):
+        check(dev, z, u, **settings)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_widest_vocabulary(dev, dtype):
+    """2048 pieces, in two rounds of a CTA's threads; masses of 38 bits."""
+    z, u = logits(1, 1 << 24, dtype, seed=24)
+    assert m.lib().mgpu_hip_sample_workspace_bytes(1, 1 << 24) > 0
+    for settings in (dict(), dict(p=0.9), dict(k=300, p=0.8)):
+        check(dev, z, u, **settings)
+    ties = torch.full_like(z, 3.0)
+    ties[0, :100] = -math.inf
+    for settings in (dict(), dict(p=0.6), dict(k=(1 << 24) - 5000)):
+        check(dev, ties, u, **settings)
