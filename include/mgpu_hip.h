@@ -354,8 +354,9 @@ MGPU_HIP_API int mgpu_hip_inner_join_pairs(int a_count, int b_count,
  *  - An output may not overlap an input, except where it says so; a matrix
  *    takes everything from its first value to its last, gaps between its rows
  *    too.
- *  - Numbers of tokens, rows of a table and values of a row go up to 2^30;
- *    more is refused. */
+ *  - Numbers of tokens and of rows of logits, values of a row, and rows of a
+ *    gradient's table go up to 2^30; more is refused.  (A table that rows are
+ *    only looked up in may have more.) */
 
 /* output[t] = scale * table[ids[t]] for t in [0, count): rows of dim values.
  * An id outside [0, num_rows) is padding and gives zeros. */
@@ -387,8 +388,9 @@ MGPU_HIP_API int mgpu_hip_embedding_grad(const void* grad,
  * (the others are padding) and q = softmax(z / temperature):
  *   loss[r] = w * temperature^2 * sum_k p_k (log p_k - log q[id_k])
  *   dz[v]   = w * temperature * (q[v] - sum of p_k over id_k == v)
- * Several entries may name one id.  A row of weight 0, or without a usable
- * entry, is not read: loss 0, gradient 0, norms 0.  A row of -inf only has
+ * Several entries may name one id.  A row of weight 0, or without an entry
+ * whose id lies in the vocabulary and whose logit is above -inf, has loss 0,
+ * gradient 0 and norms 0, whatever its logits are.  A row of -inf only has
  * q = 0; NaN or +inf in a row make its loss and gradient NaN.
  * teacher_dtype: MGPU_F32, MGPU_F16 or MGPU_BF16.  temperature > 0, finite.
  *
@@ -425,8 +427,11 @@ MGPU_HIP_API int mgpu_hip_distill_loss_and_grad(const void* logits,
  * <= 0 (or NaN) keeps the first alone; NaN as top_p or min_p keeps
  * everything.  -inf and NaN are never drawn, +inf counts as
  * the largest finite float; a row with nothing else gives token -1 and
- * logprob -inf.  Probabilities are summed as 64-bit whole numbers: the token
- * does not depend on the order of the sums.
+ * logprob -inf.  The sums that place top-p's border and the draw are of 64-bit
+ * whole numbers, multiples of 2^-38 of the largest probability or finer, and do
+ * not depend on their order.  Sums over a whole row (the total of top-p without
+ * top-k, a draw without any setting) are of 64-bit floats, added in an order
+ * that vocab alone decides.
  * Each setting is an array with a value a row or, where that is NULL, the
  * one value for all rows.  vocab in [1, MGPU_HIP_SAMPLE_MAX_VOCAB].
  * Workspace: mgpu_hip_sample_workspace_bytes. */

@@ -9,9 +9,9 @@
 // All sums, exponentials and logarithms are 32-bit; a gradient is rounded to
 // the logits' type once.
 //
-// A row without a usable teacher entry, or of weight 0, has loss 0 and
-// gradient 0 and is not read: whatever it holds does not matter.  A row whose
-// logits are all -inf has q = 0.  NaN or +inf in a row that is read makes its
+// A row without a usable teacher entry (an index in range, a logit above -inf),
+// or of weight 0, has loss 0 and gradient 0: whatever it holds does not matter,
+// and a row of weight 0 is not read.  A row whose logits are all -inf has q = 0.  NaN or +inf in a row that is read makes its
 // loss and gradient NaN.
 //
 // Row reductions beside reduce(), and a gather by column index beside spmv().

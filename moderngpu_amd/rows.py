@@ -184,8 +184,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, weights=N
     vocabulary (use -1 for padding).
 
     Returns ``(loss, norms)``, float32 with a value and with two values a row;
-    ``distill_grad`` takes the norms.  Rows of weight 0 are not read; their
-    loss and norms are 0."""
+    ``distill_grad`` takes the norms.  Rows of weight 0, or without an entry
+    that counts, have loss and norms 0, whatever their logits are."""
     matrix, teacher, w, types = _distill_args(logits, teacher_ids, teacher_logits, weights)
     lead = logits.shape[:-1]
     loss = torch.empty(lead, dtype=torch.float32, device=logits.device)
