@@ -85,9 +85,10 @@ struct embedding_lookup_f {
 // CTA waits for another's sort: the three launches below take 21.9 us for 1537
 // tokens into 10007 x 515 fp32 and 24.7 for 2048, this one 15.0 and 20.2 (bf16
 // into 1000 x 64: 28.9 and 11.2; 32768 x 1024: 25.8 and 23.3; 131072 x 4096:
-// 201 and 181).  A row of all 2048 tokens is where they are better (10007 x
-// 515: 24 against 68 us, one CTA's share of the memory): past 2048 they take
-// all.
+// 201 and 181).  A row of all 2048 tokens is where they are better, as it gets
+// one CTA's share of the memory here (whole calls, 10007 x 515: 27 us against 34
+// in fp32 and 24 against 72 in bf16; bf16 into 32768 x 4096: 59 against 127):
+// past 2048 they take all.
 enum { embedding_few = 2048 };
 
 template<typename grad_t, typename out_t, bool stream>
@@ -266,7 +267,9 @@ enum { embedding_plan_nt = 1024, embedding_plan_rows = 512,
 // tokens and counters of its own, so equal ids keep their token order.  T ids
 // are read (rows / embedding_plan_rows) times, from L2; a radix sort would
 // read them less often but takes six dependent launches for 17-bit ids.  Up to
-// 16384 tokens stay in registers between the two passes.
+// 16384 tokens stay in registers between the two passes; more are read twice,
+// and what all CTAs read grows as tokens x rows (whole calls into 65536 x 1024
+// bf16: 16384 tokens 37 us, 32768 47, 65536 72, 131072 133).
 struct embedding_plan_f {
   enum { nt = embedding_plan_nt, R = embedding_plan_rows, W = nt / 64,
     rounds = 16 };
