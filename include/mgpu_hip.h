@@ -428,8 +428,8 @@ MGPU_HIP_API int mgpu_hip_distill_loss_and_grad(const void* logits,
  * everything.  -inf and NaN are never drawn, +inf counts as
  * the largest finite float; a row with nothing else gives token -1 and
  * logprob -inf.  The sums that place top-p's border and the draw are of 64-bit
- * whole numbers, multiples of 2^-38 of the largest probability or finer, and do
- * not depend on their order.  Sums over a whole row (the total of top-p without
+ * whole numbers, multiples of 2^-38 of the largest probability or finer (2^-45
+ * for a vocab of 131072), and do not depend on their order.  Sums over a whole row (the total of top-p without
  * top-k, a draw without any setting) are of 64-bit floats, added in an order
  * that vocab alone decides.
  * Each setting is an array with a value a row or, where that is NULL, the

@@ -99,7 +99,8 @@ def _out(out, shape, dtype):
 
 def embedding_lookup(table, ids, scale=1.0, out=None):
     """out[..., :] = scale * table[ids[...]] for an int32 tensor of ids.  Ids
-    outside the table are padding and give zeros."""
+    outside the table are padding and give zeros.  Nothing is recorded for
+    autograd: embedding_grad is the gradient in the table."""
     _int32(ids, "ids")
     if table.dim() != 2:
         raise TypeError("table must be two-dimensional")
@@ -185,7 +186,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, weights=N
 
     Returns ``(loss, norms)``, float32 with a value and with two values a row;
     ``distill_grad`` takes the norms.  Rows of weight 0, or without an entry
-    that counts, have loss and norms 0, whatever their logits are."""
+    that counts, have loss and norms 0, whatever their logits are.  Nothing is
+    recorded for autograd: distill_grad is the gradient in the logits."""
     matrix, teacher, w, types = _distill_args(logits, teacher_ids, teacher_logits, weights)
     lead = logits.shape[:-1]
     loss = torch.empty(lead, dtype=torch.float32, device=logits.device)
