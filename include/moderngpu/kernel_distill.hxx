@@ -273,13 +273,20 @@ struct distill_f {
     float from = none ? 0.f : m;
     float inv_s = none ? 0.f : __builtin_amdgcn_exp2f(-log2_s);
 
-    // The entries' loss terms, and what stands in their columns.
+    // The entries' loss terms, and what stands in their columns.  A term is
+    // taken times tau and in 64 bits up to its row weight: the logit of a
+    // teacher's token that the student rules out with its type's lowest value is
+    // past the largest float once it is divided by tau, or by ln 2; the loss
+    // need not be.
     float coef = w * tau, sum = 0, column[entries];
+    double log_a = (double)tau * (log2_a * ln2),
+      log_s = (double)tau * (log2_s * ln2);
     PRAGMA_UNROLL
     for(int j = 0; j < entries; ++j) {
       if(mode != distill_grad_only && !(p[j] == 0)) {
-        float log2_q = none ? -inf : (at[j] - m) * c - log2_s;
-        sum += p[j] * ((a[j] - a_max) * c - log2_a - log2_q) * ln2;
+        double log_p = (double)a[j] - (double)a_max - log_a;
+        double log_q = none ? -inf : (double)at[j] - (double)m - log_s;
+        sum += (float)((double)coef * p[j] * (log_p - log_q));
       }
       column[j] = coef * (share(at[j], from) * inv_s - total[j]);
     }
@@ -293,7 +300,7 @@ struct distill_f {
     if(mode != distill_grad_only && !tid) {
       PRAGMA_UNROLL
       for(int i = 1; i < waves; ++i) sum += shared_reduce[i];
-      loss[row] = w * tau * tau * sum;
+      loss[row] = sum;
       if(norms) {
         norms[2 * (int64_t)row] = m;
         norms[2 * (int64_t)row + 1] = log2_s * ln2;

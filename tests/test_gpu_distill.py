@@ -341,3 +341,23 @@ def test_refusals(dev):
     wide = torch.zeros(3, 9, device=dev)
     with pytest.raises(m.MgpuError):
         m.distill_loss_and_grad(wide[:, :8], ids, a, out=wide[:, 1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tau", [0.5, 1.0, 2.0])
+def test_teachers_tokens_that_hold_the_lowest_value(dev, dtype, tau):
+    """A student that masks with its type's lowest value rules out tokens of
+    the teacher's: log q lies near or past the lowest float, the loss is
+    finite.  Weights of a mean over rows; a row that holds the largest value
+    as well."""
+    z, ids, teacher, weights = make(4, 900, 8, dtype, seed=25)
+    lowest = torch.finfo(dtype).min
+    ids[:] = torch.arange(8, dtype=torch.int32) * 100
+    teacher[:] = torch.linspace(0, 1, 8)
+    weights[:] = 2.0 ** -6
+    z[0, 100] = lowest
+    z[1, ::100] = lowest
+    z[2, 1:] = lowest
+    z[3, 300], z[3, 5] = lowest, -lowest
+    loss, _, _ = run_all(dev, z, ids, teacher, weights, tau, dtype)
+    assert bool(torch.isfinite(loss).all())
