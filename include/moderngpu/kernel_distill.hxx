@@ -286,7 +286,7 @@ struct distill_f {
       if(mode != distill_grad_only && !(p[j] == 0)) {
         double log_p = (double)a[j] - (double)a_max - log_a;
         double log_q = none ? -inf : (double)at[j] - (double)m - log_s;
-        sum += (float)((double)coef * p[j] * (log_p - log_q));
+        sum += (float)((double)w * tau * p[j] * (log_p - log_q));
       }
       column[j] = coef * (share(at[j], from) * inv_s - total[j]);
     }
